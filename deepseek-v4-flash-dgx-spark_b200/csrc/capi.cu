@@ -1053,6 +1053,184 @@ int dsv4_sparse_attn(const void* q, const void* kv, const float* attn_sink, cons
                             workspace ? workspace_bytes : 0, num_sms(), static_cast<cudaStream_t>(stream));
 }
 
+// ---- attention cache --------------------------------------------------------
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static bool rotary_shape_ok(int D, int rot, int offset) {
+  return rot >= 0 && rot % 2 == 0 && offset >= 0 && (long long)offset + rot <= D;
+}
+
+int dsv4_rotary(const void* x, void* y, int dtype, const void* positions, int pos64, const double* freqs, int B, int S,
+                int H, int D, int rot, int offset, int interleaved, int inverse, float amplitude,
+                const long long* x_strides, const long long* y_strides, void* stream) {
+  if (B < 0 || S < 0 || H < 0 || D <= 0 || !rotary_shape_ok(D, rot, offset)) return DSV4_ERR_ARG;
+  if (dtype < DSV4_DTYPE_BF16 || dtype > DSV4_DTYPE_FP32) return DSV4_ERR_UNSUPPORTED;
+  if (rot > kRotMax || D > (1 << 20)) return DSV4_ERR_UNSUPPORTED;
+  if (B == 0 || S == 0 || H == 0) return DSV4_OK;
+  if (!x || !y || !x_strides || !y_strides || (rot && (!positions || !freqs))) return DSV4_ERR_ARG;
+  for (int i = 0; i < 3; ++i)
+    if (x == y && x_strides[i] != y_strides[i]) return DSV4_ERR_ARG;
+  bind_device(y);
+  return launch_rotary(x, y, dtype, positions, pos64, freqs, B, S, H, D, rot, offset, interleaved, inverse, amplitude,
+                       x_strides, y_strides, static_cast<cudaStream_t>(stream));
+}
+
+// What every entry point on a paged cache asks of its sizes.
+static int cache_shape(int n_pages, int page_size, int n_seqs, int max_pages) {
+  if (n_pages <= 0 || page_size <= 0 || n_seqs <= 0 || max_pages <= 0) return DSV4_ERR_ARG;
+  if (page_size > 4096 || max_pages > (1 << 20) || (long long)max_pages * page_size > INT_MAX - 4096)
+    return DSV4_ERR_UNSUPPORTED;
+  return DSV4_OK;
+}
+
+// Pages as 16-byte units: rows of D 16-bit elements, a page's rows side by side.
+static int cache_rows(const void* pages, int n_layers, int page_size, int D, long long layer_stride,
+                      long long page_stride) {
+  if (!pages || n_layers <= 0 || D <= 0) return DSV4_ERR_ARG;
+  if (D % 8 || layer_stride % 8 || page_stride % 8 || !aligned16(pages)) return DSV4_ERR_UNSUPPORTED;
+  if ((long long)page_size * D > (1 << 24)) return DSV4_ERR_UNSUPPORTED;
+  return DSV4_OK;
+}
+
+int dsv4_cache_append(const void* rows, long long row_stride, int dtype, int T, int D, void* pages, int n_pages,
+                      int page_size, long long page_stride, const int* page_table, int n_seqs, int max_pages,
+                      const void* seq_ids, const void* positions, int index64, const double* freqs, int rot, int offset,
+                      int interleaved, float amplitude, void* stream) {
+  if (T < 0 || !rotary_shape_ok(D, rot, offset)) return DSV4_ERR_ARG;
+  if (dtype != DSV4_DTYPE_BF16 && dtype != DSV4_DTYPE_FP16) return DSV4_ERR_UNSUPPORTED;
+  int rc = cache_shape(n_pages, page_size, n_seqs, max_pages);
+  if (rc == DSV4_OK) rc = cache_rows(pages, 1, page_size, D, 0, page_stride);
+  if (rc != DSV4_OK) return rc;
+  if (rot > 2 * kAppendPairs) return DSV4_ERR_UNSUPPORTED;
+  if (T == 0) return DSV4_OK;
+  if (!rows || !page_table || !positions || (rot && !freqs)) return DSV4_ERR_ARG;
+  bind_device(pages);
+  return launch_cache_append(rows, row_stride, dtype, T, D, pages, n_pages, page_size, page_stride, page_table, n_seqs,
+                             max_pages, seq_ids, positions, index64, freqs, rot, offset, interleaved, amplitude,
+                             static_cast<cudaStream_t>(stream));
+}
+
+long long dsv4_cache_reserve_workspace_bytes(int n, int n_seqs, int n_pages) {
+  return n < 0 || n_seqs <= 0 || n_pages <= 0 ? -1 : cache_reserve_workspace(n, n_seqs, n_pages);
+}
+
+int dsv4_cache_reserve(int* page_table, int* seq_lens, int* page_refs, int n_seqs, int max_pages, int n_pages,
+                       int page_size, const int* seqs, const int* new_lens, int n, void* workspace,
+                       long long workspace_bytes, void* stream) {
+  if (n < 0) return DSV4_ERR_ARG;
+  const int rc = cache_shape(n_pages, page_size, n_seqs, max_pages);
+  if (rc != DSV4_OK) return rc;
+  if (n == 0) return DSV4_OK;
+  if (!page_table || !seq_lens || !page_refs || !seqs || !new_lens) return DSV4_ERR_ARG;
+  if (!workspace || workspace_bytes < cache_reserve_workspace(n, n_seqs, n_pages)) return DSV4_ERR_WORKSPACE;
+  bind_device(page_table);
+  return launch_cache_reserve(page_table, seq_lens, page_refs, n_seqs, max_pages, n_pages, page_size, seqs, new_lens, n,
+                              static_cast<int*>(workspace), static_cast<cudaStream_t>(stream));
+}
+
+int dsv4_cache_free(int* page_table, int* seq_lens, int* page_refs, int n_seqs, int max_pages, int n_pages,
+                    const int* seqs, int n, void* stream) {
+  if (n < 0) return DSV4_ERR_ARG;
+  const int rc = cache_shape(n_pages, 1, n_seqs, max_pages);
+  if (rc != DSV4_OK) return rc;
+  if (n == 0) return DSV4_OK;
+  if (!page_table || !seq_lens || !page_refs || !seqs) return DSV4_ERR_ARG;
+  bind_device(page_table);
+  return launch_cache_free(page_table, seq_lens, page_refs, n_seqs, max_pages, n_pages, seqs, n,
+                           static_cast<cudaStream_t>(stream));
+}
+
+long long dsv4_cache_fork_workspace_bytes(int n, int n_seqs) {
+  return n < 0 || n_seqs <= 0 ? -1 : cache_fork_workspace(n, n_seqs);
+}
+
+int dsv4_cache_fork(void* pages, int n_layers, int D, long long layer_stride, long long page_stride, int* page_table,
+                    int* seq_lens, int* page_refs, int n_seqs, int max_pages, int n_pages, int page_size,
+                    const int* parents, const int* children, const int* fork_lens, int n, void* workspace,
+                    long long workspace_bytes, void* stream) {
+  if (n < 0) return DSV4_ERR_ARG;
+  int rc = cache_shape(n_pages, page_size, n_seqs, max_pages);
+  if (rc == DSV4_OK) rc = cache_rows(pages, n_layers, page_size, D, layer_stride, page_stride);
+  if (rc != DSV4_OK) return rc;
+  if (n == 0) return DSV4_OK;
+  if (!page_table || !seq_lens || !page_refs || !parents || !children) return DSV4_ERR_ARG;
+  if (!workspace || workspace_bytes < cache_fork_workspace(n, n_seqs)) return DSV4_ERR_WORKSPACE;
+  bind_device(pages);
+  return launch_cache_fork(pages, n_layers, layer_stride * 2, page_stride * 2, D * 2, page_table, seq_lens, page_refs,
+                           n_seqs, max_pages, n_pages, page_size, parents, children, fork_lens, n,
+                           static_cast<int*>(workspace), static_cast<cudaStream_t>(stream));
+}
+
+long long dsv4_cache_compact_workspace_bytes(int n_pages) {
+  return n_pages <= 0 ? -1 : cache_compact_workspace(n_pages);
+}
+
+int dsv4_cache_compact(void* pages, int n_layers, int D, long long layer_stride, long long page_stride,
+                       int* page_table, int* page_refs, int n_seqs, int max_pages, int n_pages, int page_size,
+                       int* page_map, void* workspace, long long workspace_bytes, void* stream) {
+  int rc = cache_shape(n_pages, page_size, n_seqs, max_pages);
+  if (rc == DSV4_OK) rc = cache_rows(pages, n_layers, page_size, D, layer_stride, page_stride);
+  if (rc != DSV4_OK) return rc;
+  if (!page_table || !page_refs || !page_map) return DSV4_ERR_ARG;
+  if (!workspace || workspace_bytes < cache_compact_workspace(n_pages)) return DSV4_ERR_WORKSPACE;
+  bind_device(pages);
+  return launch_cache_compact(pages, n_layers, layer_stride * 2, page_stride * 2, D * 2, page_table, page_refs, n_seqs,
+                              max_pages, n_pages, page_size, page_map, static_cast<int*>(workspace), num_sms(),
+                              static_cast<cudaStream_t>(stream));
+}
+
+int dsv4_cache_copy(void* pages, int n_layers, int D, long long layer_stride, long long page_stride, int n_pages,
+                    int page_size, const int* src, const int* dst, int n, void* stream) {
+  if (n < 0) return DSV4_ERR_ARG;
+  int rc = cache_shape(n_pages, page_size, 1, 1);
+  if (rc == DSV4_OK) rc = cache_rows(pages, n_layers, page_size, D, layer_stride, page_stride);
+  if (rc != DSV4_OK) return rc;
+  if (n == 0) return DSV4_OK;
+  if (!src || !dst) return DSV4_ERR_ARG;
+  bind_device(pages);
+  return launch_cache_copy(pages, n_layers, layer_stride * 2, page_stride * 2, D * 2, n_pages, page_size, src, dst, n,
+                           static_cast<cudaStream_t>(stream));
+}
+
+static int paged_attn_shape(int T, int H, int D, int page_size, int max_pages) {
+  if (T < 0 || H <= 0 || D <= 0) return DSV4_ERR_ARG;
+  const int rc = cache_shape(1, page_size, 1, max_pages);
+  if (rc != DSV4_OK) return rc;
+  if (H > 128 || (D != 128 && D != 256 && D != 512)) return DSV4_ERR_UNSUPPORTED;
+  if (page_size < 16 || (page_size & (page_size - 1)) || T > (1 << 24)) return DSV4_ERR_UNSUPPORTED;
+  return DSV4_OK;
+}
+
+long long dsv4_paged_attn_workspace_bytes(int T, int H, int D, int page_size, int max_pages) {
+  if (paged_attn_shape(T, H, D, page_size, max_pages) != DSV4_OK) return -1;
+  return paged_attn_workspace(T, H, D, (long long)max_pages * page_size, num_sms());
+}
+
+int dsv4_paged_attn(const void* q, long long q_stride_t, long long q_stride_h, int dtype, int T, int H, int D,
+                    const void* pages, int n_pages, int page_size, long long page_stride, const int* page_table,
+                    int n_seqs, int max_pages, const void* seq_ids, const void* positions, int index64,
+                    const float* attn_sink, float softmax_scale, int window, int first, void* out, void* workspace,
+                    long long workspace_bytes, void* stream) {
+  int rc = paged_attn_shape(T, H, D, page_size, max_pages);
+  if (rc != DSV4_OK) return rc;
+  if (n_pages <= 0 || n_seqs <= 0 || window < 0 || first < 0) return DSV4_ERR_ARG;
+  if (dtype != DSV4_DTYPE_BF16 && dtype != DSV4_DTYPE_FP16) return DSV4_ERR_UNSUPPORTED;
+  if (T == 0) return DSV4_OK;
+  if (!q || !page_table || !positions || !out) return DSV4_ERR_ARG;
+  rc = cache_rows(pages, 1, page_size, D, 0, page_stride);
+  if (rc != DSV4_OK) return rc;
+  // tensor-map loads of q, 16-byte stores of rows that see nothing
+  if (!aligned16(q) || !aligned16(out) || q_stride_t % 8 || q_stride_h % 8 || q_stride_t < D || q_stride_h < D ||
+      page_stride < D)
+    return DSV4_ERR_ARG;
+  bind_device(out);
+  return launch_paged_attn(q, dtype == DSV4_DTYPE_FP16, T, H, D, q_stride_t, q_stride_h, pages, n_pages, page_size,
+                           page_stride, page_table, n_seqs, max_pages, seq_ids, positions, index64, attn_sink,
+                           softmax_scale, window, first, out, workspace, workspace ? workspace_bytes : 0, num_sms(),
+                           static_cast<cudaStream_t>(stream));
+}
+
 int dsv4_materialize(const uint8_t* slab, const long long* src_off, const int* dst_slot, int n,
                      int hidden, int inter, uint8_t* arena, long long slot_stride,
                      uint8_t* arena_sf, long long sf_slot_stride, void* bf16_out,

@@ -9,5 +9,8 @@
 #include "materialize.cu"
 #include "ep.cu"
 #include "sparse_attn.cu"
+#include "rotary.cu"
+#include "page_ops.cu"
+#include "paged_attn.cu"
 #include "capi.cu"
 #include "no_alloc.cu"

@@ -112,6 +112,36 @@ long long sparse_attn_workspace(int tokens, int K, int num_sms, int* splits_out,
 int launch_sparse_attn(const void* q, const void* kv, const float* sink, const int* idx, int B, int S,
                        int N, int K, float scale, void* out, void* ws, long long ws_bytes, int num_sms,
                        cudaStream_t st);
+// attention cache (rotary.cu, page_ops.cu, paged_attn.cu); layer and page
+// strides of the page operations are in bytes, those of the others in elements
+int launch_rotary(const void* x, void* y, int dtype, const void* positions, int pos64, const double* freqs, int B,
+                  int S, int H, int D, int rot, int offset, int interleaved, int inverse, float amplitude,
+                  const long long* xs, const long long* ys, cudaStream_t st);
+int launch_cache_append(const void* rows, long long row_stride, int dtype, int T, int D, void* pages, int n_pages,
+                        int page_size, long long page_stride, const int* table, int n_seqs, int max_pages,
+                        const void* seq_ids, const void* positions, int idx64, const double* freqs, int rot, int offset,
+                        int interleaved, float amplitude, cudaStream_t st);
+long long cache_reserve_workspace(int n, int n_seqs, int n_pages);
+long long cache_fork_workspace(int n, int n_seqs);
+long long cache_compact_workspace(int n_pages);
+int launch_cache_reserve(int* table, int* lens, int* refs, int n_seqs, int max_pages, int n_pages, int page_size,
+                         const int* seqs, const int* new_lens, int n, int* ws, cudaStream_t st);
+int launch_cache_free(int* table, int* lens, int* refs, int n_seqs, int max_pages, int n_pages, const int* seqs, int n,
+                      cudaStream_t st);
+int launch_cache_fork(void* pages, int n_layers, long long layer_stride, long long page_stride, int row_bytes,
+                      int* table, int* lens, int* refs, int n_seqs, int max_pages, int n_pages, int page_size,
+                      const int* parents, const int* children, const int* fork_lens, int n, int* ws, cudaStream_t st);
+int launch_cache_compact(void* pages, int n_layers, long long layer_stride, long long page_stride, int row_bytes,
+                         int* table, int* refs, int n_seqs, int max_pages, int n_pages, int page_size, int* page_map,
+                         int* ws, int num_sms, cudaStream_t st);
+int launch_cache_copy(void* pages, int n_layers, long long layer_stride, long long page_stride, int row_bytes,
+                      int n_pages, int page_size, const int* src, const int* dst, int n, cudaStream_t st);
+long long paged_attn_workspace(int T, int H, int D, long long max_keys, int num_sms);
+int launch_paged_attn(const void* q, bool fp16, int T, int H, int D, long long q_stride_t, long long q_stride_h,
+                      const void* pages, int n_pages, int page_size, long long page_stride, const int* table,
+                      int n_seqs, int max_pages, const void* seq_ids, const void* positions, int idx64,
+                      const float* sink, float scale, int window, int first, void* out, void* ws, long long ws_bytes,
+                      int num_sms, cudaStream_t st);
 int launch_combine(const void* O, int H, const int* route_slot, const int64_t* indices, int T,
                    int k, const int* shared_base, void* y, cudaStream_t st,
                    const void* O_shared = nullptr);

@@ -16,6 +16,7 @@
 //                         slot_stride, sf_slot_stride
 //   scalars : float[2]    route_scale, swiglu_limit
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
@@ -334,6 +335,310 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& weight, const at::T
   return y;
 }
 
+// ---- attention cache: rotary positions, pages, paged attention --------------
+
+int dtype_of(const at::Tensor& t, const char* name, bool fp32_too) {
+  if (t.scalar_type() == at::kBFloat16) return DSV4_DTYPE_BF16;
+  if (t.scalar_type() == at::kHalf) return DSV4_DTYPE_FP16;
+  TORCH_CHECK(fp32_too && t.scalar_type() == at::kFloat, name, " must be bfloat16", fp32_too ? ", float16 or float32" : " or float16");
+  return DSV4_DTYPE_FP32;
+}
+
+void check_on(const at::Tensor& t, const at::Tensor& like, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
+}
+
+// An index tensor of the given number of elements as contiguous int32 or int64.
+at::Tensor index_tensor(const at::Tensor& t, const at::Tensor& like, int64_t numel, const char* name) {
+  check_on(t, like, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
+  TORCH_CHECK(t.numel() == numel, name, " must have ", numel, " elements, has ", t.numel());
+  return t.contiguous();
+}
+
+at::Tensor int32_list(const at::Tensor& t, const at::Tensor& like, const char* name) {
+  TORCH_CHECK(t.dim() == 1, name, " must have one dimension");
+  return index_tensor(t, like, t.numel(), name).to(at::kInt);
+}
+
+int rotated_channels(const at::Tensor& freqs, const at::Tensor& like) {
+  check_on(freqs, like, "freqs");
+  TORCH_CHECK(freqs.scalar_type() == at::kDouble && freqs.dim() == 1 && freqs.is_contiguous(),
+              "freqs must be a contiguous float64 vector (radians per position of each pair)");
+  TORCH_CHECK(freqs.numel() <= 1 << 20, "freqs has too many pairs");
+  return static_cast<int>(2 * freqs.numel());
+}
+
+// x as [B, S, H, D] with D contiguous: fewer dimensions get ones in front, more are merged.
+at::Tensor four_dims(const at::Tensor& x, bool may_copy) {
+  TORCH_CHECK(x.dim() >= 2, "x must be [..., heads, dim]");
+  at::Tensor v = x;
+  while (v.dim() < 4) v = v.unsqueeze(0);
+  if (v.dim() > 4) {
+    std::vector<int64_t> shape{-1, v.size(-3), v.size(-2), v.size(-1)};
+    shape[0] = 1;
+    for (int64_t i = 0; i < v.dim() - 3; ++i) shape[0] *= v.size(i);
+    v = may_copy ? v.reshape(shape) : v.view(shape);
+  }
+  if (v.stride(-1) != 1 && v.size(-1) != 1) {
+    TORCH_CHECK(may_copy, "x must be contiguous in its last dimension");
+    v = v.contiguous();
+  }
+  return v;
+}
+
+void run_rotary(const at::Tensor& x, const at::Tensor& y, const at::Tensor& positions, const at::Tensor& freqs,
+                bool interleaved, std::optional<int64_t> offset, bool inverse, double amplitude) {
+  const int dtype = dtype_of(x, "x", true);
+  const int rot = rotated_channels(freqs, x);
+  const int64_t D = x.size(3), off = offset.value_or(D - rot);
+  TORCH_CHECK(off >= 0 && off + rot <= D, "the rotated channels do not fit into a head of ", D);
+  for (int i = 0; i < 4; ++i) TORCH_CHECK(x.size(i) <= INT32_MAX, "x is too large");
+  const at::Tensor pos = index_tensor(positions, x, x.size(0) * x.size(1), "positions");
+  if (x.numel() == 0) return;
+  c10::cuda::CUDAGuard guard(x.device());
+  long long xs[3], ys[3];
+  for (int i = 0; i < 3; ++i) {  // the stride of a dimension of one entry says nothing
+    xs[i] = x.size(i) > 1 ? x.stride(i) : 0;
+    ys[i] = x.size(i) > 1 ? y.stride(i) : 0;
+  }
+  check_status(dsv4_rotary(x.data_ptr(), y.data_ptr(), dtype, pos.data_ptr(), pos.scalar_type() == at::kLong,
+                           freqs.data_ptr<double>(), static_cast<int>(x.size(0)), static_cast<int>(x.size(1)),
+                           static_cast<int>(x.size(2)), static_cast<int>(D), rot, static_cast<int>(off), interleaved,
+                           inverse, static_cast<float>(amplitude), xs, ys, stream_of(x)),
+               "dsv4_rotary");
+}
+
+at::Tensor rotary(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
+                  std::optional<int64_t> offset, bool inverse, double amplitude) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  const at::Tensor v = four_dims(x, true);
+  at::Tensor y = at::empty(v.sizes(), v.options());
+  run_rotary(v, y, positions, freqs, interleaved, offset, inverse, amplitude);
+  return y.view(x.sizes());
+}
+
+void rotary_(at::Tensor x, const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
+             std::optional<int64_t> offset, bool inverse, double amplitude) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), "rotary_ has no gradient: use rotary");
+  TORCH_CHECK(at::has_internal_overlap(x) != at::MemOverlap::Yes, "x must not overlap itself (expanded tensor)");
+  const at::Tensor v = four_dims(x, false);
+  run_rotary(v, v, positions, freqs, interleaved, offset, inverse, amplitude);
+}
+
+// The page tensor as [L, P, page_size, D] with whole pages contiguous.
+struct Pages {
+  void* ptr;
+  int dtype, layers, n_pages, page_size, D;
+  long long layer_stride, page_stride;
+};
+
+Pages pages_of(const at::Tensor& pages, bool one_layer) {
+  TORCH_CHECK(pages.is_cuda(), "pages must be a CUDA tensor");
+  TORCH_CHECK(pages.dim() == 3 || (pages.dim() == 4 && !one_layer),
+              one_layer ? "pages must be [n_pages, page_size, dim]" : "pages must be [(layers,) n_pages, page_size, dim]");
+  const int64_t d = pages.dim();
+  TORCH_CHECK(pages.stride(d - 1) == 1 && pages.stride(d - 2) == pages.size(d - 1),
+              "the rows of a page must be contiguous");
+  TORCH_CHECK(pages.size(d - 3) > 1 ? pages.stride(d - 3) >= pages.size(d - 2) * pages.size(d - 1) : true,
+              "pages must not overlap");
+  for (int64_t i = 0; i < d; ++i) TORCH_CHECK(pages.size(i) > 0 && pages.size(i) <= INT32_MAX, "pages: bad size");
+  Pages p{};
+  p.ptr = pages.data_ptr();
+  p.dtype = dtype_of(pages, "pages", false);
+  p.layers = d == 4 ? static_cast<int>(pages.size(0)) : 1;
+  p.n_pages = static_cast<int>(pages.size(d - 3));
+  p.page_size = static_cast<int>(pages.size(d - 2));
+  p.D = static_cast<int>(pages.size(d - 1));
+  // the stride of a dimension of one entry says nothing
+  p.page_stride = p.n_pages > 1 ? pages.stride(d - 3) : static_cast<long long>(p.page_size) * p.D;
+  p.layer_stride = p.layers > 1 ? pages.stride(0) : 0;
+  TORCH_CHECK(p.layers == 1 || p.layer_stride != 0, "layers must not overlap");
+  return p;
+}
+
+struct Table {
+  int* ptr;
+  int n_seqs, max_pages;
+};
+
+Table table_of(const at::Tensor& page_table) {
+  check_cuda(page_table, "page_table");
+  TORCH_CHECK(page_table.dim() == 2 && page_table.scalar_type() == at::kInt && page_table.numel() > 0,
+              "page_table must be int32 [sequences, pages]");
+  TORCH_CHECK(page_table.size(0) <= INT32_MAX && page_table.size(1) <= INT32_MAX, "page_table: bad size");
+  return {page_table.data_ptr<int>(), static_cast<int>(page_table.size(0)), static_cast<int>(page_table.size(1))};
+}
+
+int* state_of(const at::Tensor& t, const at::Tensor& table, int64_t n, const char* name) {
+  check_cuda(t, name);
+  check_on(t, table, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && (n < 0 || t.size(0) == n) && t.numel() > 0, name,
+              " must be an int32 vector that fits the cache");
+  return t.data_ptr<int>();
+}
+
+// seq_ids (optional) and positions as one index type.
+struct RowIndex {
+  at::Tensor seqs, positions;
+  bool is64;
+};
+
+RowIndex row_index(const OptT& seq_ids, const at::Tensor& positions, const at::Tensor& like, int64_t T, int n_seqs) {
+  RowIndex r;
+  r.positions = index_tensor(positions, like, T, "positions");
+  r.is64 = r.positions.scalar_type() == at::kLong;
+  if (seq_ids.has_value())
+    r.seqs = index_tensor(*seq_ids, like, T, "seq_ids").to(r.positions.scalar_type());
+  else
+    TORCH_CHECK(T <= n_seqs, "more rows than sequences: give seq_ids");
+  return r;
+}
+
+void cache_append(at::Tensor pages, const at::Tensor& rows, const at::Tensor& page_table, const OptT& seq_ids,
+                  const at::Tensor& positions, const OptT& freqs, bool interleaved, std::optional<int64_t> offset,
+                  double amplitude) {
+  const Pages p = pages_of(pages, true);
+  const Table tb = table_of(page_table);
+  check_on(rows, pages, "rows");
+  check_on(page_table, pages, "page_table");
+  TORCH_CHECK(rows.dim() == 2 && rows.size(1) == p.D && rows.scalar_type() == pages.scalar_type(),
+              "rows must be [tokens, dim] of the type of pages");
+  TORCH_CHECK(rows.size(0) <= INT32_MAX, "too many rows");
+  const at::Tensor r = rows.stride(1) == 1 ? rows : rows.contiguous();
+  const RowIndex ix = row_index(seq_ids, positions, pages, rows.size(0), tb.n_seqs);
+  const int rot = freqs.has_value() ? rotated_channels(*freqs, pages) : 0;
+  const int64_t off = offset.value_or(p.D - rot);
+  TORCH_CHECK(off >= 0 && off + rot <= p.D, "the rotated channels do not fit into a row of ", p.D);
+  c10::cuda::CUDAGuard guard(pages.device());
+  check_status(dsv4_cache_append(r.data_ptr(), r.stride(0), p.dtype, static_cast<int>(r.size(0)), p.D, p.ptr, p.n_pages,
+                                 p.page_size, p.page_stride, tb.ptr, tb.n_seqs, tb.max_pages,
+                                 ix.seqs.defined() ? ix.seqs.data_ptr() : nullptr, ix.positions.data_ptr(), ix.is64,
+                                 freqs.has_value() ? freqs->data_ptr<double>() : nullptr, rot, static_cast<int>(off),
+                                 interleaved, static_cast<float>(amplitude), stream_of(pages)),
+               "dsv4_cache_append");
+}
+
+void cache_reserve(at::Tensor page_table, at::Tensor seq_lens, at::Tensor page_refs, const at::Tensor& seqs,
+                   const at::Tensor& lens, int64_t page_size) {
+  const Table tb = table_of(page_table);
+  int* sl = state_of(seq_lens, page_table, tb.n_seqs, "seq_lens");
+  int* refs = state_of(page_refs, page_table, -1, "page_refs");
+  c10::cuda::CUDAGuard guard(page_table.device());
+  const at::Tensor s = int32_list(seqs, page_table, "seqs"), l = int32_list(lens, page_table, "lens");
+  TORCH_CHECK(s.numel() == l.numel(), "seqs and lens must be of one length");
+  TORCH_CHECK(page_size > 0 && page_size <= 4096, "page_size must be in 1 .. 4096");
+  const int n = static_cast<int>(s.numel()), n_pages = static_cast<int>(page_refs.numel());
+  const long long need = dsv4_cache_reserve_workspace_bytes(n, tb.n_seqs, n_pages);
+  const at::Tensor ws = at::empty({std::max<long long>(need, 1)}, page_table.options().dtype(at::kByte));
+  check_status(dsv4_cache_reserve(tb.ptr, sl, refs, tb.n_seqs, tb.max_pages, n_pages, static_cast<int>(page_size),
+                                  s.data_ptr<int>(), l.data_ptr<int>(), n, ws.data_ptr(), need, stream_of(page_table)),
+               "dsv4_cache_reserve");
+}
+
+void cache_free(at::Tensor page_table, at::Tensor seq_lens, at::Tensor page_refs, const at::Tensor& seqs) {
+  const Table tb = table_of(page_table);
+  int* sl = state_of(seq_lens, page_table, tb.n_seqs, "seq_lens");
+  int* refs = state_of(page_refs, page_table, -1, "page_refs");
+  c10::cuda::CUDAGuard guard(page_table.device());
+  const at::Tensor s = int32_list(seqs, page_table, "seqs");
+  check_status(dsv4_cache_free(tb.ptr, sl, refs, tb.n_seqs, tb.max_pages, static_cast<int>(page_refs.numel()),
+                               s.data_ptr<int>(), static_cast<int>(s.numel()), stream_of(page_table)),
+               "dsv4_cache_free");
+}
+
+void cache_fork(at::Tensor pages, at::Tensor page_table, at::Tensor seq_lens, at::Tensor page_refs,
+                const at::Tensor& parents, const at::Tensor& children, const OptT& lens) {
+  const Pages p = pages_of(pages, false);
+  const Table tb = table_of(page_table);
+  check_on(page_table, pages, "page_table");
+  int* sl = state_of(seq_lens, page_table, tb.n_seqs, "seq_lens");
+  int* refs = state_of(page_refs, page_table, p.n_pages, "page_refs");
+  c10::cuda::CUDAGuard guard(pages.device());
+  const at::Tensor a = int32_list(parents, pages, "parents"), b = int32_list(children, pages, "children");
+  TORCH_CHECK(a.numel() == b.numel(), "parents and children must be of one length");
+  at::Tensor l;
+  if (lens.has_value()) {
+    l = int32_list(*lens, pages, "lens");
+    TORCH_CHECK(l.numel() == a.numel(), "lens must have an entry per child");
+  }
+  const int n = static_cast<int>(a.numel());
+  const long long need = dsv4_cache_fork_workspace_bytes(n, tb.n_seqs);
+  const at::Tensor ws = at::empty({std::max<long long>(need, 1)}, pages.options().dtype(at::kByte));
+  check_status(dsv4_cache_fork(p.ptr, p.layers, p.D, p.layer_stride, p.page_stride, tb.ptr, sl, refs, tb.n_seqs,
+                               tb.max_pages, p.n_pages, p.page_size, a.data_ptr<int>(), b.data_ptr<int>(),
+                               l.defined() ? l.data_ptr<int>() : nullptr, n, ws.data_ptr(), need, stream_of(pages)),
+               "dsv4_cache_fork");
+}
+
+at::Tensor cache_compact(at::Tensor pages, at::Tensor page_table, at::Tensor page_refs) {
+  const Pages p = pages_of(pages, false);
+  const Table tb = table_of(page_table);
+  check_on(page_table, pages, "page_table");
+  int* refs = state_of(page_refs, page_table, p.n_pages, "page_refs");
+  c10::cuda::CUDAGuard guard(pages.device());
+  at::Tensor map = at::empty({p.n_pages}, page_refs.options());
+  const long long need = dsv4_cache_compact_workspace_bytes(p.n_pages);
+  const at::Tensor ws = at::empty({std::max<long long>(need, 1)}, pages.options().dtype(at::kByte));
+  check_status(dsv4_cache_compact(p.ptr, p.layers, p.D, p.layer_stride, p.page_stride, tb.ptr, refs, tb.n_seqs,
+                                  tb.max_pages, p.n_pages, p.page_size, map.data_ptr<int>(), ws.data_ptr(), need,
+                                  stream_of(pages)),
+               "dsv4_cache_compact");
+  return map;
+}
+
+void cache_copy(at::Tensor pages, const at::Tensor& src, const at::Tensor& dst) {
+  const Pages p = pages_of(pages, false);
+  c10::cuda::CUDAGuard guard(pages.device());
+  const at::Tensor a = int32_list(src, pages, "src"), b = int32_list(dst, pages, "dst");
+  TORCH_CHECK(a.numel() == b.numel(), "src and dst must be of one length");
+  check_status(dsv4_cache_copy(p.ptr, p.layers, p.D, p.layer_stride, p.page_stride, p.n_pages, p.page_size,
+                               a.data_ptr<int>(), b.data_ptr<int>(), static_cast<int>(a.numel()), stream_of(pages)),
+               "dsv4_cache_copy");
+}
+
+at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& pages, const at::Tensor& page_table, const OptT& seq_ids,
+                      const at::Tensor& positions, const OptT& attn_sink, double softmax_scale, int64_t window,
+                      int64_t first) {
+  const Pages p = pages_of(pages, true);
+  const Table tb = table_of(page_table);
+  check_on(q, pages, "q");
+  check_on(page_table, pages, "page_table");
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == p.D && q.scalar_type() == pages.scalar_type(),
+              "q must be [tokens, heads, dim] of the type of pages");
+  TORCH_CHECK(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX, "q is too large");
+  TORCH_CHECK(window >= 0 && first >= 0, "window and first must not be negative");
+  c10::cuda::CUDAGuard guard(pages.device());
+  const int T = static_cast<int>(q.size(0)), H = static_cast<int>(q.size(1));
+  // strides that the tensor-map loads cannot take are laid out anew
+  const bool direct = q.stride(2) == 1 && (H == 1 || (q.stride(1) % 8 == 0 && q.stride(1) >= p.D)) &&
+                      (T <= 1 || (q.stride(0) % 8 == 0 && q.stride(0) >= p.D)) &&
+                      reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0;
+  const at::Tensor qc = direct ? q : q.clone(at::MemoryFormat::Contiguous);
+  const long long st = T > 1 ? qc.stride(0) : static_cast<long long>(H) * p.D, sh = H > 1 ? qc.stride(1) : p.D;
+  const RowIndex ix = row_index(seq_ids, positions, pages, T, tb.n_seqs);
+  at::Tensor sink;
+  if (attn_sink.has_value()) {
+    TORCH_CHECK(attn_sink->numel() == H, "attn_sink must have an entry per head");
+    sink = attn_sink->to(pages.device(), at::kFloat).contiguous();
+  }
+  at::Tensor out = at::empty({T, H, p.D}, q.options());
+  const long long need = dsv4_paged_attn_workspace_bytes(T, H, p.D, p.page_size, tb.max_pages);
+  if (need < 0)
+    check_status(DSV4_ERR_UNSUPPORTED, "paged_attn (1 to 128 heads; dim 128, 256 or 512; page_size a power of two from 16 on)");
+  const at::Tensor ws = at::empty({std::max<long long>(need, 1)}, pages.options().dtype(at::kByte));
+  const int64_t most = INT32_MAX;
+  check_status(dsv4_paged_attn(qc.data_ptr(), st, sh, p.dtype, T, H, p.D, p.ptr, p.n_pages, p.page_size, p.page_stride,
+                               tb.ptr, tb.n_seqs, tb.max_pages, ix.seqs.defined() ? ix.seqs.data_ptr() : nullptr,
+                               ix.positions.data_ptr(), ix.is64, sink.defined() ? sink.data_ptr<float>() : nullptr,
+                               static_cast<float>(softmax_scale), static_cast<int>(std::min(window, most)),
+                               static_cast<int>(std::min(first, most)), out.data_ptr(), ws.data_ptr(), need,
+                               stream_of(pages)),
+               "dsv4_paged_attn");
+  return out;
+}
+
 // ---------------------------------------------------------- arena / materializer
 int64_t materialize(const at::Tensor& slab, const at::Tensor& src_off, const at::Tensor& dst_slot,
                     const OptT& arena, int64_t slot_stride, const OptT& arena_sf, int64_t sf_slot_stride,
@@ -551,6 +856,21 @@ TORCH_LIBRARY(dsv4moe, m) {
   m.def("sparse_attn(Tensor q, Tensor kv, Tensor attn_sink, Tensor topk_idxs, float softmax_scale) -> Tensor");
   m.def("build_fp8_weight_atoms(Tensor scale, int out_features, int in_features) -> Tensor");
   m.def("fp8_linear(Tensor x, Tensor weight, Tensor weight_atoms) -> Tensor");
+  m.def("rotary(Tensor x, Tensor positions, Tensor freqs, bool interleaved=True, int? offset=None, "
+        "bool inverse=False, float amplitude=1.0) -> Tensor");
+  m.def("rotary_(Tensor(a!) x, Tensor positions, Tensor freqs, bool interleaved=True, int? offset=None, "
+        "bool inverse=False, float amplitude=1.0) -> ()");
+  m.def("cache_append(Tensor(a!) pages, Tensor rows, Tensor page_table, Tensor? seq_ids, Tensor positions, "
+        "Tensor? freqs=None, bool interleaved=True, int? offset=None, float amplitude=1.0) -> ()");
+  m.def("cache_reserve(Tensor(a!) page_table, Tensor(b!) seq_lens, Tensor(c!) page_refs, Tensor seqs, Tensor lens, "
+        "int page_size) -> ()");
+  m.def("cache_free(Tensor(a!) page_table, Tensor(b!) seq_lens, Tensor(c!) page_refs, Tensor seqs) -> ()");
+  m.def("cache_fork(Tensor(a!) pages, Tensor(b!) page_table, Tensor(c!) seq_lens, Tensor(d!) page_refs, "
+        "Tensor parents, Tensor children, Tensor? lens=None) -> ()");
+  m.def("cache_compact(Tensor(a!) pages, Tensor(b!) page_table, Tensor(c!) page_refs) -> Tensor");
+  m.def("cache_copy(Tensor(a!) pages, Tensor src, Tensor dst) -> ()");
+  m.def("paged_attn(Tensor q, Tensor pages, Tensor page_table, Tensor? seq_ids, Tensor positions, "
+        "Tensor? attn_sink, float softmax_scale, int window=0, int first=0) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(dsv4moe, CUDA, m) {
@@ -574,6 +894,15 @@ TORCH_LIBRARY_IMPL(dsv4moe, CUDA, m) {
   m.impl("sparse_attn", &sparse_attn);
   m.impl("build_fp8_weight_atoms", &build_fp8_weight_atoms);
   m.impl("fp8_linear", &fp8_linear);
+  m.impl("rotary", &rotary);
+  m.impl("rotary_", &rotary_);
+  m.impl("cache_append", &cache_append);
+  m.impl("cache_reserve", &cache_reserve);
+  m.impl("cache_free", &cache_free);
+  m.impl("cache_fork", &cache_fork);
+  m.impl("cache_compact", &cache_compact);
+  m.impl("cache_copy", &cache_copy);
+  m.impl("paged_attn", &paged_attn);
 }
 
 // Ops without tensor inputs on a device (sizes, host reads) dispatch here.

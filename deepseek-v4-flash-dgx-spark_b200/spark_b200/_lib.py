@@ -43,6 +43,8 @@ DEVERR_NAMES = {
     105: "routing plan exceeds its workspace",
     106: "materializer source offset not 16-byte aligned",
     107: "a peer rank's exchange flag did not arrive in time",
+    108: "cache sequence, position, length or page out of range",
+    109: "cache out of free pages",
 }
 
 
@@ -91,6 +93,22 @@ _SIGNATURES = {
     "dsv4_sparse_attn_workspace_bytes": (c_ll, [c_int, c_int, c_int]),
     "dsv4_sparse_attn": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
                                  c_vp, c_vp, c_ll, c_vp]),
+    "dsv4_rotary": (c_int, [c_vp, c_vp, c_int, c_vp, c_int, c_vp] + [c_int] * 8 + [c_float, c_llp, c_llp, c_vp]),
+    "dsv4_cache_append": (c_int, [c_vp, c_ll, c_int, c_int, c_int, c_vp, c_int, c_int, c_ll, c_vp, c_int, c_int, c_vp,
+                                  c_vp, c_int, c_vp, c_int, c_int, c_int, c_float, c_vp]),
+    "dsv4_cache_reserve_workspace_bytes": (c_ll, [c_int, c_int, c_int]),
+    "dsv4_cache_reserve": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_ll, c_vp]),
+    "dsv4_cache_free": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_int, c_vp]),
+    "dsv4_cache_fork_workspace_bytes": (c_ll, [c_int, c_int]),
+    "dsv4_cache_fork": (c_int, [c_vp, c_int, c_int, c_ll, c_ll, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp,
+                                c_vp, c_vp, c_int, c_vp, c_ll, c_vp]),
+    "dsv4_cache_compact_workspace_bytes": (c_ll, [c_int]),
+    "dsv4_cache_compact": (c_int, [c_vp, c_int, c_int, c_ll, c_ll, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp,
+                                   c_ll, c_vp]),
+    "dsv4_cache_copy": (c_int, [c_vp, c_int, c_int, c_ll, c_ll, c_int, c_int, c_vp, c_vp, c_int, c_vp]),
+    "dsv4_paged_attn_workspace_bytes": (c_ll, [c_int] * 5),
+    "dsv4_paged_attn": (c_int, [c_vp, c_ll, c_ll, c_int, c_int, c_int, c_int, c_vp, c_int, c_int, c_ll, c_vp, c_int,
+                                c_int, c_vp, c_vp, c_int, c_vp, c_float, c_int, c_int, c_vp, c_vp, c_ll, c_vp]),
     "dsv4_moe_workspace_bytes": (c_ll, [ctypes.POINTER(MoELayerDesc), c_int]),
     "dsv4_moe_workspace_layout": (c_int, [ctypes.POINTER(MoELayerDesc), c_int, c_llp, c_int]),
     "dsv4_moe_forward": (c_int, [ctypes.POINTER(MoELayerDesc), c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_ll, c_vp]),

@@ -50,6 +50,13 @@ extern "C" {
 #define DSV4_DEVERR_PLAN_OVERFLOW 105
 #define DSV4_DEVERR_MISALIGNED 106  /* a materializer source offset is not 16-byte aligned */
 #define DSV4_DEVERR_TIMEOUT_PEER 107  /* a peer rank's exchange flag did not arrive within 2 s */
+#define DSV4_DEVERR_BAD_CACHE_INDEX 108 /* a cache operation's sequence, position, length or page is out of range */
+#define DSV4_DEVERR_NO_PAGES 109        /* a cache operation needed more free pages than there are */
+
+/* element types of the attention cache entry points */
+#define DSV4_DTYPE_BF16 0
+#define DSV4_DTYPE_FP16 1
+#define DSV4_DTYPE_FP32 2
 
 DSV4_API int dsv4_version(void);
 /* Number of kernels the library has enqueued in this process (every launch
@@ -283,6 +290,104 @@ DSV4_API long long dsv4_sparse_attn_workspace_bytes(int B, int S, int K);
 DSV4_API int dsv4_sparse_attn(const void* q, const void* kv, const float* attn_sink, const int* topk_idxs,
                               int B, int S, int H, int N, int D, int K, float softmax_scale, void* out,
                               void* workspace, long long workspace_bytes, void* stream);
+
+/* ---- attention cache ------------------------------------------------------
+ * The operators a decode loop runs around the attention (the reference keeps
+ * positions and cache inside the official model; these entry points have no
+ * counterpart among its files).
+ *
+ * Rotary positions: for pair i of the `rot` channels from `offset` on, with
+ * angle = position * freqs[i] (freqs: device double [rot/2], radians per
+ * position),
+ *     y[c] = (x[c] cos - x[c'] sin) * amplitude,  y[c'] = (x[c'] cos + x[c] sin) * amplitude
+ * (c, c') = offset + (2i, 2i+1) if interleaved, else offset + (i, i + rot/2).
+ * inverse != 0 rotates by -angle: the transposed map, hence the gradient's.
+ * Other channels pass through.  Angles are reduced in 64 bits.
+ * x, y: [B,S,H,D] of dtype BF16, FP16 or FP32; strides of (b, s, h) in
+ * elements, D contiguous; positions [B,S], int32 or (pos64) int64.  y == x with
+ * equal strides rotates in place and touches the rotated channels only; any
+ * other overlap is undefined.  rot <= 4096. */
+DSV4_API int dsv4_rotary(const void* x, void* y, int dtype, const void* positions, int pos64, const double* freqs,
+                         int B, int S, int H, int D, int rot, int offset, int interleaved, int inverse,
+                         float amplitude, const long long* x_strides, const long long* y_strides, void* stream);
+
+/* A paged cache: pages [P][page_size][D] of 16-bit elements (a page's rows side
+ * by side, page_stride elements from page to page; 16-byte aligned, D % 8 == 0),
+ * in n_layers layers layer_stride elements apart that share the page ids;
+ * page_table int32 [n_seqs][max_pages] (pages of a sequence in order, -1 behind
+ * the last), seq_lens int32 [n_seqs] (tokens a sequence has room for), page_refs
+ * int32 [n_pages] (sequences that hold a page; 0 = free).  Tables live on the
+ * device and change in stream order; nothing is read back.  Bad entries are
+ * skipped and latch DSV4_DEVERR_BAD_CACHE_INDEX.
+ *
+ * append: row t of rows [T,D] (row_stride elements apart) is rotated (rot = 0:
+ * not) and written as row positions[t] of sequence seq_ids[t] (NULL: sequence
+ * t).  index64: seq_ids and positions are int64, else int32.  A negative
+ * sequence or position marks padding and is skipped.  No two rows may name the
+ * same place (either row's bytes may end up there).  rot <= 512. */
+DSV4_API int dsv4_cache_append(const void* rows, long long row_stride, int dtype, int T, int D, void* pages,
+                               int n_pages, int page_size, long long page_stride, const int* page_table, int n_seqs,
+                               int max_pages, const void* seq_ids, const void* positions, int index64,
+                               const double* freqs, int rot, int offset, int interleaved, float amplitude,
+                               void* stream);
+/* reserve: sequence seqs[i] gets room for new_lens[i] tokens (never less than it
+ * has): free pages, lowest id first, in the order of the entries.  If there are
+ * too few, nothing changes and DSV4_DEVERR_NO_PAGES is latched.  A negative
+ * sequence is padding; a sequence named again is a bad entry. */
+DSV4_API long long dsv4_cache_reserve_workspace_bytes(int n, int n_seqs, int n_pages);
+DSV4_API int dsv4_cache_reserve(int* page_table, int* seq_lens, int* page_refs, int n_seqs, int max_pages,
+                                int n_pages, int page_size, const int* seqs, const int* new_lens, int n,
+                                void* workspace, long long workspace_bytes, void* stream);
+/* free: the sequences' pages lose a holder each, their table rows and lengths
+ * are cleared.  A negative sequence is padding, one named again is freed once. */
+DSV4_API int dsv4_cache_free(int* page_table, int* seq_lens, int* page_refs, int n_seqs, int max_pages, int n_pages,
+                             const int* seqs, int n, void* stream);
+/* fork: the empty sequence children[i] becomes the first fork_lens[i] tokens
+ * (NULL: all) of parents[i].  Full pages are shared; a part-filled last page is
+ * copied to a free page (lowest id first) in every layer, so either side may go
+ * on writing behind the fork.  A child that holds tokens or is named again, or a
+ * length beyond the parent's, is a bad entry; a negative id is padding; too few
+ * free pages change nothing. */
+DSV4_API long long dsv4_cache_fork_workspace_bytes(int n, int n_seqs);
+DSV4_API int dsv4_cache_fork(void* pages, int n_layers, int D, long long layer_stride, long long page_stride,
+                             int* page_table, int* seq_lens, int* page_refs, int n_seqs, int max_pages, int n_pages,
+                             int page_size, const int* parents, const int* children, const int* fork_lens, int n,
+                             void* workspace, long long workspace_bytes, void* stream);
+/* compact: the used pages move to the ids 0 .. used-1 in every layer (a used
+ * page below that stays; the k-th free id below takes the k-th used page above),
+ * tables and holder counts follow.  page_map int32 [n_pages]: each old id's new
+ * one, -1 for a free page. */
+DSV4_API long long dsv4_cache_compact_workspace_bytes(int n_pages);
+DSV4_API int dsv4_cache_compact(void* pages, int n_layers, int D, long long layer_stride, long long page_stride,
+                                int* page_table, int* page_refs, int n_seqs, int max_pages, int n_pages,
+                                int page_size, int* page_map, void* workspace, long long workspace_bytes,
+                                void* stream);
+/* copy: page src[i] to page dst[i] in every layer.  A negative id is padding.
+ * An entry whose target is another entry's source or an earlier one's target is
+ * a bad entry. */
+DSV4_API int dsv4_cache_copy(void* pages, int n_layers, int D, long long layer_stride, long long page_stride,
+                             int n_pages, int page_size, const int* src, const int* dst, int n, void* stream);
+
+/* Attention of single tokens over a paged cache whose rows serve every head as
+ * key and value: q [T,H,D] (strides in elements, D contiguous), row t stands at
+ * positions[t] of sequence seq_ids[t] (NULL: sequence t),
+ *     out[t,h] = sum_j p[h,j] kv[j],  p = softmax(softmax_scale * q[t,h].kv[j])
+ * over the keys j <= positions[t], with window > 0 only those above
+ * positions[t] - window and the first `first` ones, and with exp(attn_sink[h])
+ * (NULL: none) in the denominator.  Keys on no page are left out and latch
+ * DSV4_DEVERR_BAD_CACHE_INDEX.  A row with a negative sequence or position, or
+ * with no key, gives zeros.  What hidden rows of a page hold (NaN included) has
+ * no effect.  out [T,H,D].
+ * H <= 128; D = 128, 256 or 512; page_size a power of two from 16 on; BF16 or
+ * FP16; all 16-byte aligned (DSV4_ERR_UNSUPPORTED / DSV4_ERR_ARG otherwise).
+ * Two calls may share a workspace only if they do not overlap on the GPU. */
+DSV4_API long long dsv4_paged_attn_workspace_bytes(int T, int H, int D, int page_size, int max_pages);
+DSV4_API int dsv4_paged_attn(const void* q, long long q_stride_t, long long q_stride_h, int dtype, int T, int H,
+                             int D, const void* pages, int n_pages, int page_size, long long page_stride,
+                             const int* page_table, int n_seqs, int max_pages, const void* seq_ids,
+                             const void* positions, int index64, const float* attn_sink, float softmax_scale,
+                             int window, int first, void* out, void* workspace, long long workspace_bytes,
+                             void* stream);
 
 /* ---- expert arena / materializer ---------------------------------------
  * LazyRoutedExpert.materialize + ExpertCopyPlan::read_into_and_copy_cuda
