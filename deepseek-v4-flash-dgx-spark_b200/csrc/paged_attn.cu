@@ -44,6 +44,7 @@ constexpr int kPaTile = kPaChunk * 128;           // 16 KB: 128 rows x 64 channe
 constexpr int kPaMaxStages = 12;
 constexpr int kPaCtrl = 2048;
 constexpr int kPaSmemMax = 232448;                // shared memory a CTA may use
+constexpr int kPaMaxGrid = 1024;                  // CTAs (one per SM)
 constexpr int kPaTmemCols = 512;                  // S: two buffers of 64 columns; O^T at 256
 constexpr float kPaRescaleLog = 8.0f;             // headroom of the running max (natural log)
 
@@ -653,44 +654,112 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   }
 }
 
-// Join the pieces of a row that crosses CTA borders.  Block (c, h): border c lies
-// inside a row and is its first; the row's pieces are CTA c - 1's second kind (the
-// one that holds the row's begin) and the first kind of CTAs c .. last.
+// Join the pieces of the rows that cross CTA borders.  Border c (CTA c begins inside
+// a row) is a row's first if the row begins in CTA c - 1; the row's pieces are then
+// CTA c - 1's second kind (the one that holds its begin) and the first kind of CTAs
+// c, c + 1, ...  Every CTA lists those rows from the plan, and the work units (row,
+// head, 128 channels) go round the warps of the grid: one warp per unit, or all
+// eight of a CTA, each on every eighth piece, where the units are few (one long row
+// left in 65 pieces: 64 heads x 4 units).
+constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinAhead = 8;  // pieces whose loads are in flight together
+
 template <typename T, int N>
-__global__ void __launch_bounds__(128) paged_attn_join_kernel(const PaArgs a) {
-  const int c = blockIdx.x + 1, h = blockIdx.y;
-  const int4 pl = a.plan[c];  // row, group, chunks before the border, chunks of the row
+__global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaArgs a, int n_plan) {
+  __shared__ int4 rows[kPaMaxGrid];   // row, head group, first piece, pieces
+  __shared__ int count[kJoinWarps];
+  __shared__ float red[kJoinWarps][32][4];
+  __shared__ float den_of[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long share = *a.share;
-  if (pl.x < 0 || pl.z == 0 || pl.z > share) return;
-  const int t = pl.x, g = pl.y;
-  if (64 * g + h >= a.H) return;
-  const int n_parts = 2 + (int)((pl.w - pl.z - 1) / share);
-  const size_t p0 = (size_t)(c - 1) * 2;  // parts: p0 + 1, p0 + 2, p0 + 4, ...
-  auto piece = [&](int i) { return p0 + (i == 0 ? 1 : 2 * i); };
-  const float sk = a.sink ? __ldg(a.sink + 64 * g + h) : -INFINITY;
-  float mx = sk;
-  for (int i = 0; i < n_parts; ++i) mx = fmaxf(mx, a.part_ml[(piece(i) * N + h) * 2]);
-  float den = sk == -INFINITY ? 0.f : __expf(sk - mx);
-  bool any = false;
-  for (int i = 0; i < n_parts; ++i) {
-    const float m = a.part_ml[(piece(i) * N + h) * 2];
-    if (m == -INFINITY) continue;
-    any = true;
-    den += a.part_ml[(piece(i) * N + h) * 2 + 1] * __expf(m - mx);
-  }
-  for (int d = threadIdx.x; d < a.D; d += blockDim.x) {
-    float acc = 0.f;
-    for (int i = 0; i < n_parts; ++i) {
-      const float m = a.part_ml[(piece(i) * N + h) * 2];
-      if (m > -INFINITY) acc += a.part_o[(piece(i) * N + h) * a.D + d] * __expf(m - mx);
+  int n_rows = 0;  // in border order, so that every CTA has the same list
+  for (int base = 1; base < n_plan; base += kJoinThreads) {
+    const int c = base + threadIdx.x;
+    int4 pl = make_int4(-1, 0, 0, 0);  // row, group, chunks before the border, chunks of the row
+    if (c < n_plan) pl = a.plan[c];
+    const bool on = pl.x >= 0 && pl.z > 0 && pl.z <= share;
+    const unsigned vote = __ballot_sync(0xffffffffu, on);
+    if (lane == 0) count[warp] = __popc(vote);
+    __syncthreads();
+    int at = n_rows;
+    for (int w = 0; w < kJoinWarps; ++w) {
+      if (w < warp) at += count[w];
+      n_rows += count[w];
     }
-    static_cast<T*>(a.out)[((size_t)t * a.H + 64 * g + h) * a.D + d] = from_f32<T>(any ? acc / den : 0.f);
+    if (on) rows[at + __popc(vote & ((1u << lane) - 1))] = make_int4(pl.x, pl.y, c - 1, 2 + (int)((pl.w - pl.z - 1) / share));
+    __syncthreads();
+  }
+  const int slices = a.D / 128;
+  const long long units = (long long)n_rows * N * slices;
+  const bool together = units * kJoinWarps <= (long long)gridDim.x * kJoinWarps;
+  const long long first = together ? blockIdx.x : (long long)blockIdx.x * kJoinWarps + warp;
+  const long long step = together ? gridDim.x : (long long)gridDim.x * kJoinWarps;
+  for (long long u = first; u < units; u += step) {
+    const int slice = (int)(u % slices), h = (int)(u / slices % N);
+    const int4 r = rows[u / slices / N];
+    const int head = 64 * r.y + h;
+    if (head >= a.H) continue;
+    auto piece = [&](int i) { return (size_t)r.z * 2 + (i == 0 ? 1 : 2 * i); };
+    // each lane holds the maxima and sums of pieces lane, lane + 32, ...
+    const float sk = a.sink ? __ldg(a.sink + head) : -INFINITY;
+    float mx = sk;
+    for (int i = lane; i < r.w; i += 32) mx = fmaxf(mx, a.part_ml[(piece(i) * N + h) * 2]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float den = 0.f, acc[4] = {};
+    const int p0 = together ? warp : 0, ps = together ? kJoinWarps : 1;
+    for (int i0 = p0; i0 < r.w; i0 += ps * kJoinAhead) {
+      float4 o[kJoinAhead];
+      float f[kJoinAhead];
+#pragma unroll
+      for (int j = 0; j < kJoinAhead; ++j) {
+        const int i = i0 + j * ps;
+        f[j] = 0.f;
+        if (i >= r.w) continue;
+        const size_t at = piece(i) * N + h;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+        o[j] = *reinterpret_cast<const float4*>(a.part_o + at * a.D + 128 * slice + 4 * lane);
+        if (ml.x > -INFINITY) {
+          f[j] = __expf(ml.x - mx);
+          den += ml.y * f[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kJoinAhead; ++j) {
+        if (f[j] == 0.f) continue;
+        acc[0] += o[j].x * f[j];
+        acc[1] += o[j].y * f[j];
+        acc[2] += o[j].z * f[j];
+        acc[3] += o[j].w * f[j];
+      }
+    }
+    if (together) {
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < 4; ++x) red[warp][lane][x] = acc[x];
+      if (lane == 0) den_of[warp] = den;
+      __syncthreads();
+      if (warp) continue;
+      for (int w = 1; w < kJoinWarps; ++w) {
+        den += den_of[w];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[x] += red[w][lane][x];
+      }
+    }
+    const bool any = den > 0.f || den != den;
+    if (sk > -INFINITY) den += __expf(sk - mx);
+    Pack<T, 4> out;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) out.v[x] = from_f32<T>(any ? acc[x] / den : 0.f);
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + ((size_t)r.x * a.H + head) * a.D + 128 * slice + 4 * lane) =
+        *reinterpret_cast<const uint2*>(&out);
   }
 }
 
 // ---------------------------------------------------------------- host side
 struct PaShape {
-  int N, groups, stages, grid;
+  int N, groups, stages, grid, join_grid;
   size_t smem;
 };
 
@@ -706,7 +775,12 @@ static PaShape pa_shape(int T, int H, int D, long long max_keys, int num_sms) {
   s.stages &= ~1;  // two tiles of one 128-channel output block lie side by side
   s.smem = (size_t)fixed + (size_t)s.stages * kPaTile;
   const long long most = (long long)T * s.groups * ((max_keys + kPaChunk - 1) / kPaChunk);
+  if (num_sms > kPaMaxGrid) num_sms = kPaMaxGrid;
   s.grid = (int)(most < num_sms ? (most < 1 ? 1 : most) : num_sms);
+  // a unit per warp for every row that may be split, up to eight CTAs per SM
+  const long long split = s.grid - 1 < (long long)T * s.groups ? s.grid - 1 : (long long)T * s.groups;
+  const long long units = split * s.N * (D / 128);
+  s.join_grid = (int)(units < 8LL * num_sms ? (units < 1 ? 1 : units) : 8LL * num_sms);
   return s;
 }
 
@@ -738,7 +812,7 @@ static int launch_paged_attn_t(const PaShape& s, const CUtensorMap& qm, const CU
                                cudaStream_t st) {
   if (ensure_smem_attr(reinterpret_cast<const void*>(paged_attn_kernel<T, N>), (int)s.smem)) return DSV4_ERR_CUDA;
   launch_k(paged_attn_kernel<T, N>, s.grid, kPaThreads, s.smem, st, qm, kvm, a);
-  if (s.grid > 1) launch_k(paged_attn_join_kernel<T, N>, dim3(s.grid - 1, N), 128, 0, st, a);
+  if (s.grid > 1) launch_k(paged_attn_join_kernel<T, N>, s.join_grid, kJoinThreads, 0, st, a, s.grid);
   return cudaGetLastError() == cudaSuccess ? DSV4_OK : DSV4_ERR_CUDA;
 }
 
