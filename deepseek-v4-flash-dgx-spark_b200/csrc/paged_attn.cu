@@ -46,7 +46,9 @@ constexpr int kPaCtrl = 2048;
 constexpr int kPaSmemMax = 232448;                // shared memory a CTA may use
 constexpr int kPaMaxGrid = 1024;                  // CTAs (one per SM)
 constexpr int kPaTmemCols = 512;                  // S: two buffers of 64 columns; O^T at 256
-constexpr float kPaRescaleLog = 8.0f;             // headroom of the running max (natural log)
+constexpr float kPaRescaleLog2 = 10.0f;           // headroom of the running max, base 2
+constexpr float kPaNoMax = -3.402823466e38f;      // running max of a piece before its first key
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct PaArgs {
   void* out;              // [T, H, D]
@@ -133,6 +135,12 @@ __device__ __forceinline__ bool soft_or(bool v) {
   return r != 0;
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // n consecutive fp32 columns of this thread's TMEM lane, n = 8, 16 or 32.
 template <int n>
 __device__ __forceinline__ void tmem_ldn(uint32_t taddr, float (&v)[n]) {
@@ -203,9 +211,9 @@ __device__ __forceinline__ float warp_reduce_n(float (&v)[n], int lane) {
 
 // kind::f16 instruction descriptor: A and B both fp16 or both bf16, fp32 D, M = 128.
 template <typename T>
-__host__ __device__ constexpr uint32_t pa_idesc(uint32_t n, uint32_t a_mn) {
+__host__ __device__ constexpr uint32_t pa_idesc(uint32_t n, uint32_t a_mn, uint32_t b_mn) {
   const uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0u : 1u;
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
 __device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z) {
@@ -222,6 +230,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map,
                       const PaArgs a) {
   constexpr int HPT = N / 2;  // heads per softmax thread
+  const float scale2 = a.scale * kLog2e;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int KT = a.D / 64, DT = a.D / 128, NST = a.stages;
@@ -373,7 +382,11 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   } else if (warp == 1) {
     // ---------------------------------------------------------- products
     if (lane == 0) {
-      const uint32_t id_qk = pa_idesc<T>(N, 0), id_pv = pa_idesc<T>(N, 1);
+      constexpr uint32_t id_qk = pa_idesc<T>(N, 0, 0), id_pv = pa_idesc<T>(N, 1, N == 64);
+      // descriptors of the first tile; an address moves the low field by bytes / 16
+      const uint64_t dk = sdesc_k_sw128(smem_u32(ring)), dm = sdesc_mn_sw128(smem_u32(ring), kPaTile);
+      const uint64_t dq = sdesc_k_sw128(smem_u32(sQ));
+      const uint64_t dp = N == 64 ? sdesc_mn_sw128(smem_u32(sP), kPaTile) : sdesc_k_sw128(smem_u32(sP));
       long long left = sh.left;
       const long long chunks = left;
       // with room for two chunks the next chunk's scores are issued before this one's output
@@ -422,8 +435,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           ok = pa_wait(sh, &sh.full[slot], phase, DSV4_DEVERR_TIMEOUT_MMA);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t ad = sdesc_k_sw128(smem_u32(ring + slot * kPaTile));
-          const uint64_t bd = sdesc_k_sw128(smem_u32(sQ + kt * N * 128));
+          const uint64_t ad = dk + slot * (kPaTile / 16), bd = dq + kt * (N * 128 / 16);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             tc_mma_f16(t_s + 64 * b, ad + 2 * kk, bd + 2 * kk, id_qk, (kt | kk) ? 1u : 0u);
@@ -448,14 +460,11 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         for (int dt = 0; dt < DT; ++dt) {
           // channels 128 dt .. +127 are tiles 2 dt and 2 dt + 1 of the chunk, side by
           // side in the ring (its length is even)
-          const uint32_t a0 = smem_u32(ring + pv_slot * kPaTile);
-          for (int jt = 0; jt < kPaChunk / 64; ++jt) {
+          const uint64_t ad = dm + pv_slot * (kPaTile / 16);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              const uint64_t ad = sdesc_mn_sw128(a0 + (64 * jt + 16 * kk) * 128, kPaTile);
-              const uint64_t bd = sdesc_k_sw128(smem_u32(sP + jt * N * 128)) + 2 * kk;
-              tc_mma_f16(t_o + N * dt, ad, bd, id_pv, (!begin || jt || kk) ? 1u : 0u);
-            }
+          for (int kk = 0; kk < kPaChunk / 16; ++kk) {
+            const uint64_t bd = N == 64 ? dp + kk * (16 * 128 / 16) : dp + (kk >> 2) * (N * 128 / 16) + 2 * (kk & 3);
+            tc_mma_f16(t_o + N * dt, ad + kk * (16 * 128 / 16), bd, id_pv, (!begin || kk) ? 1u : 0u);
           }
           tc_commit(&sh.empty[pv_slot]);
           tc_commit(&sh.empty[pv_slot + 1]);
@@ -501,13 +510,11 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       const int i_begin = i, i1 = (int)min((long long)r.n, i + left);
       if (i < i1) {
         const int* pages = a.table + (long long)r.s * a.max_pages;
-        float m_run[HPT], l_run[HPT];
+        float l_run[HPT];
 #pragma unroll
-        for (int x = 0; x < HPT; ++x) {
-          m_run[x] = -INFINITY;
-          l_run[x] = 0.f;
-        }
-        if (st < N) sh.m[st] = -INFINITY;
+        for (int x = 0; x < HPT; ++x) l_run[x] = 0.f;
+        if (st < N) sh.m[st] = kPaNoMax;
+        soft_sync();
         left -= i1 - i;
         auto page_at = [&](int c) -> int {
           const int key = pa_key0(r, c) + row;
@@ -531,11 +538,14 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.s_free[b]);
-          bool raise = false;
+          float over = -INFINITY;  // how far the scores exceed the running max
+          if (valid) {
 #pragma unroll
-          for (int x = 0; x < HPT; ++x) {
-            z[x] = valid ? z[x] * a.scale : -INFINITY;
-            raise |= z[x] > m_run[x] + kPaRescaleLog;
+            for (int x = 0; x < HPT; x += 4) {
+              const float4 m4 = *reinterpret_cast<const float4*>(&sh.m[h0 + x]);
+              over = fmaxf(over, fmaxf(fmaf(z[x], scale2, -m4.x), fmaf(z[x + 1], scale2, -m4.y)));
+              over = fmaxf(over, fmaxf(fmaf(z[x + 2], scale2, -m4.z), fmaf(z[x + 3], scale2, -m4.w)));
+            }
           }
           if (!valid) {
             // whatever lies in the hidden row must not reach the output product (0 x NaN):
@@ -549,47 +559,64 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           }
           // the previous chunk's output product has read P and written O
           if (k > 0) pa_wait(sh, &sh.pv_done, (uint32_t)(k - 1) & 1, DSV4_DEVERR_TIMEOUT_EPILOGUE);
-          if (soft_or(raise)) {
+          if (soft_or(over > kPaRescaleLog2)) {
+            // raise every head's max to its largest score so far
             tc_fence_after();
             float v[HPT];
 #pragma unroll
-            for (int x = 0; x < HPT; ++x) v[x] = z[x];
-            const float mx = warp_reduce_n<HPT, false>(v, lane);
-            if (lane < HPT) sh.red[q4 * 64 + h0 + lane] = mx;
+            for (int x = 0; x < HPT; ++x) v[x] = valid ? z[x] * scale2 : -INFINITY;
+            const float top = warp_reduce_n<HPT, false>(v, lane);
+            if (lane < HPT) sh.red[q4 * 64 + h0 + lane] = top;
             soft_sync();
             if (st < N) {
               const float cm = fmaxf(fmaxf(sh.red[st], sh.red[64 + st]), fmaxf(sh.red[128 + st], sh.red[192 + st]));
               const float mo = sh.m[st], mn = fmaxf(mo, cm);
-              sh.f[st] = mo == -INFINITY ? 0.f : __expf(mo - mn);
+              sh.f[st] = ex2(mo - mn);
               sh.m[st] = mn;
             }
             soft_sync();
-            float alpha[HPT];
 #pragma unroll
-            for (int x = 0; x < HPT; ++x) {
-              alpha[x] = sh.f[h0 + x];
-              m_run[x] = sh.m[h0 + x];
-              l_run[x] *= alpha[x];
-            }
+            for (int x = 0; x < HPT; ++x) l_run[x] *= sh.f[h0 + x];
             if (i > i_begin) {
               for (int dt = 0; dt < DT; ++dt) {
                 float o[HPT];
                 tmem_ldn<HPT>(t_o + N * dt + h0 + lane_base, o);
 #pragma unroll
-                for (int x = 0; x < HPT; ++x) o[x] *= alpha[x];
+                for (int x = 0; x < HPT; ++x) o[x] *= sh.f[h0 + x];
                 tmem_stn<HPT>(t_o + N * dt + h0 + lane_base, o);
               }
               tmem_wait_st();
             }
           }
-          // P[h][j], rounded to the cache's type as the product takes it; the sum
-          // adds the rounded values, so the weights still sum to one
+          // weights, rounded to the cache's type as the product takes them; the sum adds
+          // them unrounded (their rounding errors average out over the keys)
+          if constexpr (N == 64) {
+            // P[j][h], heads contiguous: 128-byte rows, 128-byte swizzle (MN-major operand)
+            uint8_t* prow = sP + row * 128;
 #pragma unroll
-          for (int x = 0; x < HPT; ++x) {
-            const float e = z[x] == -INFINITY ? 0.f : __expf(z[x] - m_run[x]);
-            const T pb = from_f32<T>(e);
-            l_run[x] += to_f32(pb);
-            *reinterpret_cast<T*>(sP + sw128_offset(N, h0 + x, row)) = pb;
+            for (int x = 0; x < HPT; x += 8) {
+              Pack<T, 8> w;
+#pragma unroll
+              for (int y = 0; y < 8; y += 4) {
+                const float4 m4 = *reinterpret_cast<const float4*>(&sh.m[h0 + x + y]);
+                const float mm[4] = {m4.x, m4.y, m4.z, m4.w};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  const float e = valid ? ex2(fmaf(z[x + y + c], scale2, -mm[c])) : 0.f;
+                  l_run[x + y + c] += e;
+                  w.v[y + c] = from_f32<T>(e);
+                }
+              }
+              store_pack<T, 8>(reinterpret_cast<T*>(prow + ((((h0 + x) >> 3) ^ (row & 7)) << 4)), w);
+            }
+          } else {
+            // P[h][j], keys contiguous (K-major operand): 16 or 8 heads per thread
+#pragma unroll
+            for (int x = 0; x < HPT; ++x) {
+              const float e = valid ? ex2(fmaf(z[x], scale2, -sh.m[h0 + x])) : 0.f;
+              l_run[x] += e;
+              *reinterpret_cast<T*>(sP + sw128_offset(N, h0 + x, row)) = from_f32<T>(e);
+            }
           }
           fence_proxy_async_shared();
           tc_fence_before();
@@ -611,10 +638,10 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           const float l = (sh.red[st] + sh.red[64 + st]) + (sh.red[128 + st] + sh.red[192 + st]);
           const float m = sh.m[st];
           if (whole) {
-            const float sk = a.sink && st < heads ? __ldg(a.sink + 64 * g + st) : -INFINITY;
+            const float sk = a.sink && st < heads ? __ldg(a.sink + 64 * g + st) * kLog2e : -INFINITY;
             const float mx = fmaxf(m, sk);
-            const float den = l * __expf(m - mx) + (sk == -INFINITY ? 0.f : __expf(sk - mx));
-            sh.f[st] = m == -INFINITY ? 0.f : __expf(m - mx) / den;
+            const float den = l * ex2(m - mx) + ex2(sk - mx);
+            sh.f[st] = m == kPaNoMax ? 0.f : ex2(m - mx) / den;
           } else {
             a.part_ml[(piece * N + st) * 2] = m;
             a.part_ml[(piece * N + st) * 2 + 1] = l;
@@ -702,7 +729,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaA
     if (head >= a.H) continue;
     auto piece = [&](int i) { return (size_t)r.z * 2 + (i == 0 ? 1 : 2 * i); };
     // each lane holds the maxima and sums of pieces lane, lane + 32, ...
-    const float sk = a.sink ? __ldg(a.sink + head) : -INFINITY;
+    const float sk = a.sink ? __ldg(a.sink + head) * kLog2e : -INFINITY;
     float mx = sk;
     for (int i = lane; i < r.w; i += 32) mx = fmaxf(mx, a.part_ml[(piece(i) * N + h) * 2]);
 #pragma unroll
@@ -720,8 +747,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaA
         const size_t at = piece(i) * N + h;
         const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
         o[j] = *reinterpret_cast<const float4*>(a.part_o + at * a.D + 128 * slice + 4 * lane);
-        if (ml.x > -INFINITY) {
-          f[j] = __expf(ml.x - mx);
+        if (ml.x != kPaNoMax) {
+          f[j] = ex2(ml.x - mx);
           den += ml.y * f[j];
         }
       }
@@ -748,7 +775,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaA
       }
     }
     const bool any = den > 0.f || den != den;
-    if (sk > -INFINITY) den += __expf(sk - mx);
+    den += ex2(sk - mx);
     Pack<T, 4> out;
 #pragma unroll
     for (int x = 0; x < 4; ++x) out.v[x] = from_f32<T>(any ? acc[x] / den : 0.f);
