@@ -9,26 +9,36 @@
 // j % page_size of page page_table[s][j / page_size]; one cache row is key and
 // value of every head.  A row with nothing visible gives zeros.
 //
-// As in sparse_attn.cu the two products put the cache rows on the M side:
-//   S^T[j,h] = C[j,:] . Q[h,:]     M = 128 rows, N = heads, K = D
-//   O^T[d,h] += C^T[d,j] . P[h,j]  M = 128 of D, N = heads, K = 128 rows
-// and the second product reads the same shared memory as an MN-major operand.
+// Per chunk of 64 keys two products on tcgen05 (kind::f16, fp32 accumulators in TMEM):
+//   S[h,j]   = Q[h,:] . C[j,:]      M = 64 heads, N = 64 keys, K = D
+//   O^T[d,h] += C^T[d,j] . P[h,j]   M = 128 of D, N = heads, K = 64 keys
+// The second reads the same shared memory as an MN-major operand, so a key's row
+// is loaded once and never transposed.  With S's rows on heads a thread keeps two
+// heads' running max and sum in registers and takes their scores from one
+// tcgen05.ld.16x256b (M = 64 fills 16 lanes of each TMEM quarter).
 //
-// Bound: a row of D = 512 is 1 KB from HBM and 131 kFLOP with 64 heads, so the
-// cache streams at the HBM rate if the tensor core sustains 830 TFLOP/s.
+// Bound: a row of D = 512 is 1 KB from HBM and 131 kFLOP with 64 heads.  Issued
+// from warp-uniform code the two products cost 36 and 51 cycles per instruction
+// (measured), 1970 cycles per chunk, against 2840 at which an SM's share of HBM
+// delivers the chunk's 64 KB: the cache can stream at the HBM rate as long as the
+// loads never pause.  Chunks of 128 keys cost fewer tensor cycles per key but hold
+// all of the ring until their softmax is done: the loads then stand still for half
+// of the time (measured: 353 against 291 us for 16 rows of up to 131072 keys).
 //
-// Work split: the visible chunks of 128 keys of all rows form one list, and the
-// list is cut into equal shares, one per CTA (at most one CTA per SM).  Every CTA
-// finds its share from the lengths on the device, so ragged batches fill the SMs,
-// nothing is read back and a captured graph follows the lengths of each replay.
-// A row that crosses a border leaves fp32 partials (max, sum, O) that
-// paged_attn_join_kernel merges; every CTA has at most two such pieces.
+// Work split: the visible keys of all rows, in boxes of up to 64 keys on one page,
+// form one list, and the list is cut into equal shares, one per CTA (one CTA per
+// SM).  Every CTA finds its share from the lengths on the device, so ragged
+// batches fill the SMs, nothing is read back and a captured graph follows the
+// lengths of each replay.  A row that crosses a border leaves fp32 partials (max,
+// sum, O) that paged_attn_join_kernel merges; every CTA has at most two such pieces.
 //
 // Warp roles (320 threads): warp 0 loads Q and the pages by TMA into a ring of
-// [128 rows][64 channels] tiles, warp 1 issues the products, warps 2-9 do the
-// softmax: warp w reads TMEM lane quarter w % 4 (lane = cache row in the scores,
-// = channel in the output) and half of the heads.  A tile goes back to the ring
-// as soon as the output product that reads it last is done.
+// stages (64 keys x 128 channels, 16 KB), warp 1 issues the products, warps 2-9 do
+// the softmax: warp w takes the heads of TMEM quarter w % 4 and half of the chunk's
+// keys, and at the end the channels of that quarter and half of the heads.  The
+// scores of chunk k + 1 are issued as its stages arrive; the output product of
+// chunk k goes in between as soon as its weights are there, and gives its stages
+// back one by one.
 #include <limits.h>
 
 #include <type_traits>
@@ -37,10 +47,11 @@
 
 namespace dsv4 {
 
-constexpr int kPaChunk = 128;
+constexpr int kPaChunk = 64;                      // keys per chunk
 constexpr int kPaThreads = 320;
 constexpr int kPaSoft = 256;                      // softmax threads: warps 2-9
-constexpr int kPaTile = kPaChunk * 128;           // 16 KB: 128 rows x 64 channels
+constexpr int kPaTile = kPaChunk * 128;           // 8 KB: 64 keys x 64 channels, 128-byte swizzled
+constexpr int kPaStage = 2 * kPaTile;             // 16 KB: 64 keys x 128 channels
 constexpr int kPaMaxStages = 12;
 constexpr int kPaCtrl = 2048;
 constexpr int kPaSmemMax = 232448;                // shared memory a CTA may use
@@ -57,51 +68,73 @@ struct PaArgs {
   const void* positions;  // [T]
   const float* sink;      // [H] or NULL
   float* part_o;          // [grid][2][N][D]
-  float* part_ml;         // [grid][2][N][2]: max, sum
-  int4* plan;             // [grid]: row, head group, chunks of the row before this CTA, chunks of the row
-  int* share;             // [1] chunks per CTA
+  float* part_ml;         // [grid][2][N][2]: max (base 2), sum
+  int4* plan;             // [grid]: row, head group, boxes of the row before this CTA, boxes of the row
+  int* share;             // [1] boxes per CTA
   int T, H, D, groups;
-  int n_seqs, max_pages, n_pages, page_size;
+  int n_seqs, max_pages, n_pages, page_log, box_log;
   int idx64, window, first, stages, min_share;
   float scale;
 };
 
-// What row t sees: keys [w_lo, p] and [0, f).  Chunk i of its n covers the keys
-// from 128 * (i < nf ? i : i - nf + wb).
+// What row t sees: keys [w_lo, p] and [0, f), in n boxes of 1 << box_log keys; box b
+// covers the keys from (b < nfb ? b : b - nfb + wbb) << box_log.
 struct PaRow {
-  int s, p, w_lo, f, nf, wb, n;
+  int s, p, w_lo, f, nfb, wbb, n;
 };
 
-__device__ __forceinline__ PaRow pa_row(const PaArgs& a, int t) {
+// Sequence and position of row t (negative: padding).
+__device__ __forceinline__ int2 pa_index(const PaArgs& a, int t) {
+  if (t >= a.T) return make_int2(-1, -1);
+  return make_int2(a.seq_ids ? load_index(a.seq_ids, a.idx64, t) : t, load_index(a.positions, a.idx64, t));
+}
+
+__device__ __forceinline__ PaRow pa_row(const PaArgs& a, int2 sp) {
   PaRow r{};
-  r.s = a.seq_ids ? load_index(a.seq_ids, a.idx64, t) : t;
-  r.p = load_index(a.positions, a.idx64, t);
+  r.s = sp.x;
+  r.p = sp.y;
   if (r.s < 0 || r.p < 0) return r;
-  if (r.s >= a.n_seqs || r.p / a.page_size >= a.max_pages) {
+  if (r.s >= a.n_seqs || (r.p >> a.page_log) >= a.max_pages) {
     record_error(DSV4_DEVERR_BAD_CACHE_INDEX);
     return r;
   }
   r.w_lo = a.window > 0 ? max(0, r.p - a.window + 1) : 0;
   r.f = min(a.first, r.w_lo);
-  r.wb = r.w_lo / kPaChunk;
-  r.nf = min((r.f + kPaChunk - 1) / kPaChunk, r.wb);
-  r.n = r.nf + r.p / kPaChunk + 1 - r.wb;
+  r.wbb = r.w_lo >> a.box_log;
+  r.nfb = min((r.f + (1 << a.box_log) - 1) >> a.box_log, r.wbb);
+  r.n = r.nfb + (r.p >> a.box_log) + 1 - r.wbb;
   return r;
 }
-__device__ __forceinline__ int pa_key0(const PaRow& r, int i) { return kPaChunk * (i < r.nf ? i : i - r.nf + r.wb); }
+__device__ __forceinline__ int pa_box_key(const PaArgs& a, const PaRow& r, int b) {
+  return (b < r.nfb ? b : b - r.nfb + r.wbb) << a.box_log;
+}
 
 struct PaShared {
   uint64_t full[kPaMaxStages], empty[kPaMaxStages];
-  uint64_t q_full, q_empty, s_full[2], s_free[2], p_ready, pv_done, last;
+  uint64_t q_full[4], q_empty, s_full[2], s_free[2], p_ready[2], pv_done[2], last;
   uint32_t tmem;
   int abort;
-  int t0, g0, i0;           // this CTA's first row, head group and chunk
-  long long left;           // chunks of its share
+  int t0, g0, i0;           // this CTA's first row, head group and box
+  long long left;           // boxes of its share
   long long scan[kPaThreads / 32 + 1];
-  float red[4 * 64];        // one value per lane quarter and head
-  float m[64], f[64];       // running max, factor
+  float red[2 * 64];        // one value per key half and head
+  float m[64], f[64];       // max, factor per head
 };
 static_assert(sizeof(PaShared) <= kPaCtrl, "control block too small");
+
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ bool pa_aborted(PaShared& sh) { return *reinterpret_cast<volatile int*>(&sh.abort) != 0; }
 
 // A bounded wait.  Once any wait of the CTA has run out, every wait returns at
 // once: the roles run through their loops without waiting (loading and issuing
@@ -110,7 +143,7 @@ __device__ __forceinline__ bool pa_wait(PaShared& sh, uint64_t* bar, uint32_t pa
   for (int i = 0; i < 64; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer();
-  while (*reinterpret_cast<volatile int*>(&sh.abort) == 0) {
+  while (!pa_aborted(sh)) {
     for (int i = 0; i < 64; ++i)
       if (mbar_try_wait(bar, parity)) return true;
     if (globaltimer() - t0 > kWaitTimeoutNs) {
@@ -182,38 +215,25 @@ __device__ __forceinline__ void tmem_stn(uint32_t taddr, const float (&v)[n]) {
   }
 }
 
-// Reduce n values per lane over the warp's 32 lanes (max, or sum): whole
-// exchanges while a lane's half would be empty, then recursive halving.  Lane l
-// gets the reduction of value l % n.
-template <int n, bool kSum>
-__device__ __forceinline__ float warp_reduce_n(float (&v)[n], int lane) {
+// 32 columns of 16 TMEM lanes: v[4c + 0, 1] are columns 8c + 2 (lane % 4) + 0, 1 of TMEM
+// lane lane / 4, v[4c + 2, 3] the same columns eight lanes further.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+               "tcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    if (o >= n) {
-#pragma unroll
-      for (int i = 0; i < n; ++i) {
-        const float r = __shfl_xor_sync(0xffffffffu, v[i], o);
-        v[i] = kSum ? v[i] + r : fmaxf(v[i], r);
-      }
-    } else {
-      const bool up = (lane & o) != 0;
-#pragma unroll
-      for (int i = 0; i < o; ++i) {
-        const float send = up ? v[i] : v[i + o];
-        const float keep = up ? v[i + o] : v[i];
-        const float r = __shfl_xor_sync(0xffffffffu, send, o);
-        v[i] = kSum ? keep + r : fmaxf(keep, r);
-      }
-    }
-  }
-  return v[0];
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// kind::f16 instruction descriptor: A and B both fp16 or both bf16, fp32 D, M = 128.
+// kind::f16 instruction descriptor: A and B both fp16 or both bf16, fp32 D.
 template <typename T>
-__host__ __device__ constexpr uint32_t pa_idesc(uint32_t n, uint32_t a_mn, uint32_t b_mn) {
-  const uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0u : 1u;
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+__host__ __device__ constexpr uint32_t pa_idesc(uint32_t m, uint32_t n, uint32_t a_mn) {
+  const uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
 __device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z) {
@@ -224,35 +244,47 @@ __device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const CUtensorMap* 
       : "memory");
 }
 
-// N: heads per group, padded to 16, 32 or 64 (rows past H load as zeros).
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const T a = from_f32<T>(lo), b = from_f32<T>(hi);
+  uint16_t x, y;
+  memcpy(&x, &a, 2);
+  memcpy(&y, &b, 2);
+  return (uint32_t)x | ((uint32_t)y << 16);
+}
+
+// N: heads per group, padded to 16, 32 or 64 (rows past H load as zeros).  The score
+// product always takes 64 rows of Q: with N < 64 those past N are whatever follows
+// in shared memory, and no one reads their scores.
 template <typename T, int N>
 __global__ void __launch_bounds__(kPaThreads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map,
                       const PaArgs a) {
-  constexpr int HPT = N / 2;  // heads per softmax thread
-  const float scale2 = a.scale * kLog2e;
+  constexpr int HPT = N / 2;  // heads per thread of the output
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int KT = a.D / 64, DT = a.D / 128, NST = a.stages;
-  uint8_t* ring = smem;                             // NST tiles of [128 rows][128 B]
-  uint8_t* sQ = ring + NST * kPaTile;               // KT tiles of [N heads][128 B]
-  uint8_t* sP = sQ + KT * N * 128;                  // 2 tiles of [N heads][128 B]
+  const int DT = a.D / 128, NST = a.stages;
+  uint8_t* sQ = smem;                               // 2 DT tiles of [N heads][128 B]
+  uint8_t* ring = sQ + DT * 2 * N * 128;            // NST stages of two tiles [64 keys][128 B]
+  uint8_t* sP = ring + NST * kPaStage;              // 2 buffers of [N heads][64 keys]
   PaShared& sh = *reinterpret_cast<PaShared*>(sP + 2 * N * 128);
+  const int nsub = kPaChunk >> a.box_log;           // boxes per chunk
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   if (tid == 0) {
     for (int i = 0; i < NST; ++i) {
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], 1);
     }
-    mbar_init(&sh.q_full, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&sh.q_full[i], 1);
     mbar_init(&sh.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.s_free[i], kPaSoft / 32);
+      mbar_init(&sh.p_ready[i], kPaSoft / 32);
+      mbar_init(&sh.pv_done[i], 1);
     }
-    mbar_init(&sh.p_ready, kPaSoft / 32);
-    mbar_init(&sh.pv_done, 1);
     mbar_init(&sh.last, 1);
     fence_barrier_init();
     sh.abort = 0;
@@ -263,12 +295,12 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     tmem_relinquish();
   }
 
-  // ---- this CTA's share of the chunk list -----------------------------------
+  // ---- this CTA's share of the box list -------------------------------------
   {
     const int per = (a.T + kPaThreads - 1) / kPaThreads;
     const int r0 = min(a.T, tid * per), r1 = min(a.T, r0 + per);
     long long mine = 0;
-    for (int t = r0; t < r1; ++t) mine += (long long)pa_row(a, t).n * a.groups;
+    for (int t = r0; t < r1; ++t) mine += (long long)pa_row(a, pa_index(a, t)).n * a.groups;
     long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -294,7 +326,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     long long at = sh.scan[warp] + inc - mine;
     if (begin < end && at <= begin && begin < at + mine) {
       for (int t = r0; t < r1; ++t) {
-        const int n = pa_row(a, t).n;
+        const int n = pa_row(a, pa_index(a, t)).n;
         if (begin < at + (long long)n * a.groups) {
           sh.t0 = t;
           sh.g0 = (int)((begin - at) / n);
@@ -314,51 +346,77 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t t_s = sh.tmem, t_o = sh.tmem + 256;
+  const uint32_t t_s = __shfl_sync(0xffffffffu, sh.tmem, 0), t_o = t_s + 256;
+  long long left = __shfl_sync(0xffffffffu, sh.left, 0);
+  int t = __shfl_sync(0xffffffffu, sh.t0, 0), g = __shfl_sync(0xffffffffu, sh.g0, 0);
+  int i = __shfl_sync(0xffffffffu, sh.i0, 0);
+  int2 sp = left > 0 ? pa_index(a, t) : make_int2(-1, -1);  // the row at hand; the next one's is loaded early
 
   if (warp == 0) {
     // ------------------------------------------------------------- loads
-    const int rb = min(a.page_size, kPaChunk), nsub = kPaChunk / rb;  // rows per box, boxes per tile
-    long long left = sh.left;
-    int t = sh.t0, g = sh.g0, i = sh.i0;
     int slot = 0, issued = 0;
     uint32_t phase = 0, q_phase = 0;
     bool ok = true, q_issued = false;
     while (left > 0 && ok && t < a.T) {
-      const PaRow r = pa_row(a, t);
+      const PaRow r = pa_row(a, sp);
+      const int2 sp_next = pa_index(a, t + 1);
       const int i1 = (int)min((long long)r.n, i + left);
       if (i < i1) {
-        ok = __all_sync(0xffffffffu, pa_wait(sh, &sh.q_empty, q_phase ^ 1, DSV4_DEVERR_TIMEOUT_PRODUCER));
-        if (!ok) break;
-        q_phase ^= 1;
-        q_issued = true;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&sh.q_full, KT * N * 128);
-          for (int kt = 0; kt < KT; ++kt)
-            tma_load_3d_at(smem_u32(sQ + kt * N * 128), &q_map, &sh.q_full, 64 * kt, 64 * g, t);
-        }
         const int* row = a.table + (long long)r.s * a.max_pages;
         left -= i1 - i;
-        for (; i < i1 && ok; ++i) {
-          // lane b loads box b of every tile: rows key .. key + rb - 1, on one page
-          const int key = pa_key0(r, i) + lane * rb;
-          int page = -1;
-          if (lane < nsub && key <= r.p) page = __ldg(row + key / a.page_size);
-          const bool on = page >= 0 && page < a.n_pages;
-          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * rb * 128;
-          for (int kt = 0; kt < KT; ++kt) {
+        // lane b loads box b of the chunk; hidden keys and keys on no page are left out
+        auto page_at = [&](int b) -> int {
+          if (lane >= nsub || b >= i1) return -1;
+          const int page = __ldg(row + (pa_box_key(a, r, b) >> a.page_log));
+          return page < a.n_pages ? page : -1;
+        };
+        auto load_q = [&]() {
+          ok = __all_sync(0xffffffffu, pa_wait(sh, &sh.q_empty, q_phase ^ 1, DSV4_DEVERR_TIMEOUT_PRODUCER));
+          if (!ok) return;
+          q_phase ^= 1;
+          q_issued = true;
+          if (lane < DT) {
+            mbar_arrive_expect_tx(&sh.q_full[lane], 2 * N * 128);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              tma_load_3d_at(smem_u32(sQ + (2 * lane + x) * N * 128), &q_map, &sh.q_full[lane], 128 * lane + 64 * x, 64 * g, t);
+          }
+          __syncwarp();
+        };
+        // the first piece takes Q first; later ones a chunk of keys first, while the
+        // score products of the piece before may still read Q
+        bool q_due = true;
+        if (!q_issued) {
+          load_q();
+          q_due = false;
+        }
+        int page = page_at(i + lane);
+        for (; i < i1 && ok; i += nsub) {
+          const int key = pa_box_key(a, r, i + lane);
+          const bool on = page >= 0;
+          const int page_now = page;
+          page = page_at(i + nsub + lane);
+          const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, on)) * (256u << a.box_log);
+          for (int dt = 0; dt < DT; ++dt) {
             ok = __all_sync(0xffffffffu, pa_wait(sh, &sh.empty[slot], phase ^ 1, DSV4_DEVERR_TIMEOUT_PRODUCER));
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], bytes);
             __syncwarp();
-            if (on)
-              tma_load_3d_at(smem_u32(ring + slot * kPaTile) + lane * rb * 128, &kv_map, &sh.full[slot], 64 * kt,
-                             key % a.page_size, page);
+            if (on) {
+              const uint32_t dst = smem_u32(ring + slot * kPaStage) + (lane << (a.box_log + 7));
+              const int y = key & ((1 << a.page_log) - 1);
+              tma_load_3d_at(dst, &kv_map, &sh.full[slot], 128 * dt, y, page_now);
+              tma_load_3d_at(dst + kPaTile, &kv_map, &sh.full[slot], 128 * dt + 64, y, page_now);
+            }
             ++issued;
             if (++slot == NST) {
               slot = 0;
               phase ^= 1;
             }
+          }
+          if (q_due && ok) {
+            load_q();
+            q_due = false;
           }
         }
       }
@@ -366,6 +424,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       if (++g >= a.groups) {
         g = 0;
         ++t;
+        sp = sp_next;
       }
     }
     // every copy has landed before the CTA can exit, also when a wait ran out
@@ -377,207 +436,224 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       --slot;
       mbar_wait(&sh.full[slot], phase, DSV4_DEVERR_TIMEOUT_PRODUCER);
     }
-    if (q_issued) mbar_wait(&sh.q_full, q_phase ^ 1, DSV4_DEVERR_TIMEOUT_PRODUCER);
+    if (q_issued)
+      for (int k = 0; k < DT; ++k) mbar_wait(&sh.q_full[k], q_phase ^ 1, DSV4_DEVERR_TIMEOUT_PRODUCER);
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------- products
-    if (lane == 0) {
-      constexpr uint32_t id_qk = pa_idesc<T>(N, 0, 0), id_pv = pa_idesc<T>(N, 1, N == 64);
-      // descriptors of the first tile; an address moves the low field by bytes / 16
-      const uint64_t dk = sdesc_k_sw128(smem_u32(ring)), dm = sdesc_mn_sw128(smem_u32(ring), kPaTile);
-      const uint64_t dq = sdesc_k_sw128(smem_u32(sQ));
-      const uint64_t dp = N == 64 ? sdesc_mn_sw128(smem_u32(sP), kPaTile) : sdesc_k_sw128(smem_u32(sP));
-      long long left = sh.left;
-      const long long chunks = left;
-      // with room for two chunks the next chunk's scores are issued before this one's output
-      const bool ahead = NST >= 2 * KT;
-      int t = sh.t0, g = sh.g0, i = sh.i0, n = 0;  // walk of the score products
-      int i1 = 0;
-      bool fresh_q = false;
-      int slot = 0, pv_slot = 0;
-      uint32_t phase = 0, q_phase = 0;
-      long long qk_done = 0;
-      bool ok = true;
-      // the first chunk of a row (or of this share) starts its output anew
-      uint64_t begins = 0;  // bit k % 64: chunk k begins a piece
-      auto scores = [&]() {
-        while (i >= i1) {  // next piece
-          if (n) {
-            i = 0;
-            if (++g >= a.groups) {
-              g = 0;
-              ++t;
+    // All lanes run the loops, so that descriptors stay in uniform registers; one issues.
+    const bool el = elect_one();
+    constexpr uint32_t id_qk = pa_idesc<T>(64, kPaChunk, 0), id_pv = pa_idesc<T>(128, N, 1);
+    // descriptors of the first tile; an address moves the low field by bytes / 16
+    const uint64_t dq = sdesc_k_sw128(smem_u32(sQ)), dk = sdesc_k_sw128(smem_u32(ring));
+    const uint64_t dm = sdesc_mn_sw128(smem_u32(ring), kPaTile), dp = sdesc_k_sw128(smem_u32(sP));
+    bool ok = true;
+    uint32_t k_qk = 0, k_pv = 0;  // chunks whose products are issued
+    uint32_t begins = 0;          // bit k % 32: chunk k begins a piece, its output starts anew
+    int slot = 0, pv_slot = 0;
+    uint32_t phase = 0, q_phase = 0;
+
+    auto issue_pv = [&]() {
+      tc_fence_after();
+      const uint32_t b = k_pv & 1;
+      const uint32_t begin = (begins >> (k_pv & 31)) & 1;
+      for (int dt = 0; dt < DT; ++dt) {
+        if (el) {
+          const uint64_t ad = dm + pv_slot * (kPaStage / 16), bd = dp + b * (N * 128 / 16);
+#pragma unroll
+          for (int kk = 0; kk < kPaChunk / 16; ++kk)
+            tc_mma_f16(t_o + N * dt, ad + kk * (16 * 128 / 16), bd + 2 * kk, id_pv, (begin && kk == 0) ? 0u : 1u);
+          tc_commit(&sh.empty[pv_slot]);
+        }
+        if (++pv_slot == NST) pv_slot = 0;
+      }
+      if (el) tc_commit(&sh.pv_done[b]);
+      ++k_pv;
+    };
+    // Wait for a barrier; an output product whose weights get ready meanwhile is issued.
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      uint64_t t0 = 0;
+      for (uint32_t n = 1; ok; ++n) {
+        if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) break;
+        if (k_pv < k_qk && __all_sync(0xffffffffu, mbar_test_wait(&sh.p_ready[k_pv & 1], (k_pv >> 1) & 1))) issue_pv();
+        if ((n & 255) == 0) {
+          const uint64_t now = globaltimer();
+          if (t0 == 0) t0 = now;
+          if (now - t0 > kWaitTimeoutNs && lane == 0) {
+            record_error(DSV4_DEVERR_TIMEOUT_MMA);
+            *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+          }
+          __syncwarp();
+          ok = !__any_sync(0xffffffffu, pa_aborted(sh));
+        }
+      }
+    };
+    auto pv_blocking = [&]() {
+      wait(&sh.p_ready[k_pv & 1], (k_pv >> 1) & 1);
+    };
+
+    while (left > 0 && ok && t < a.T) {
+      const int n = __shfl_sync(0xffffffffu, pa_row(a, sp).n, 0);
+      const int2 sp_next = pa_index(a, t + 1);
+      const int i1 = (int)min((long long)n, i + left);
+      if (i < i1) {
+        left -= i1 - i;
+        bool begin = true;
+        for (; i < i1 && ok; i += nsub) {
+          const uint32_t b = k_qk & 1;
+          wait(&sh.s_free[b], ((k_qk >> 1) & 1) ^ 1);
+          for (int dt = 0; dt < DT && ok; ++dt) {
+            if (begin) wait(&sh.q_full[dt], q_phase);
+            wait(&sh.full[slot], phase);
+            if (!ok) break;
+            tc_fence_after();
+            if (el) {
+              const uint64_t ad = dq + dt * (2 * N * 128 / 16), bd = dk + slot * (kPaStage / 16);
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                tc_mma_f16(t_s + 64 * b, ad + (kk >> 2) * (N * 128 / 16) + 2 * (kk & 3),
+                           bd + (kk >> 2) * (kPaTile / 16) + 2 * (kk & 3), id_qk, (dt || kk) ? 1u : 0u);
+            }
+            if (++slot == NST) {
+              slot = 0;
+              phase ^= 1;
             }
           }
-          if (t >= a.T) {
-            ok = false;
-            return;
-          }
-          n = pa_row(a, t).n;
-          i1 = (int)min((long long)n, i + left);
-          if (n == 0) {
-            g = a.groups - 1;
-            n = 1;
-            i = i1 = 0;
-          } else {
-            fresh_q = true;
-          }
-        }
-        const int b = (int)(qk_done & 1);
-        const uint32_t u = (uint32_t)(qk_done >> 1) & 1;
-        if (fresh_q) {
-          ok = ok && pa_wait(sh, &sh.q_full, q_phase, DSV4_DEVERR_TIMEOUT_MMA);
-          q_phase ^= 1;
-        }
-        ok = ok && pa_wait(sh, &sh.s_free[b], u ^ 1, DSV4_DEVERR_TIMEOUT_MMA);
-        tc_fence_after();
-        for (int kt = 0; kt < KT && ok; ++kt) {
-          ok = pa_wait(sh, &sh.full[slot], phase, DSV4_DEVERR_TIMEOUT_MMA);
           if (!ok) break;
-          tc_fence_after();
-          const uint64_t ad = dk + slot * (kPaTile / 16), bd = dq + kt * (N * 128 / 16);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16(t_s + 64 * b, ad + 2 * kk, bd + 2 * kk, id_qk, (kt | kk) ? 1u : 0u);
-          if (++slot == NST) {
-            slot = 0;
-            phase ^= 1;
+          if (el) {
+            tc_commit(&sh.s_full[b]);
+            if (i + nsub >= i1) tc_commit(&sh.q_empty);  // the piece's last use of Q
+          }
+          begins = begin ? begins | (1u << (k_qk & 31)) : begins & ~(1u << (k_qk & 31));
+          begin = false;
+          ++k_qk;
+          // at most one chunk's output waits while the next scores are issued
+          if (k_qk - k_pv > 1) {
+            const uint32_t due = k_pv;
+            pv_blocking();
+            if (ok && k_pv == due) issue_pv();
           }
         }
-        if (ok) tc_commit(&sh.s_full[b]);
-        begins = fresh_q ? begins | (1ull << (qk_done & 63)) : begins & ~(1ull << (qk_done & 63));
-        fresh_q = false;
-        ++i;
-        --left;
-        if (ok && i >= i1) tc_commit(&sh.q_empty);  // the piece's last use of Q
-        ++qk_done;
-      };
-      auto outputs = [&](long long k) {
-        ok = ok && pa_wait(sh, &sh.p_ready, (uint32_t)k & 1, DSV4_DEVERR_TIMEOUT_MMA);
-        if (!ok) return;
-        tc_fence_after();
-        const bool begin = (begins >> (k & 63)) & 1;
-        for (int dt = 0; dt < DT; ++dt) {
-          // channels 128 dt .. +127 are tiles 2 dt and 2 dt + 1 of the chunk, side by
-          // side in the ring (its length is even)
-          const uint64_t ad = dm + pv_slot * (kPaTile / 16);
-#pragma unroll
-          for (int kk = 0; kk < kPaChunk / 16; ++kk) {
-            const uint64_t bd = N == 64 ? dp + kk * (16 * 128 / 16) : dp + (kk >> 2) * (N * 128 / 16) + 2 * (kk & 3);
-            tc_mma_f16(t_o + N * dt, ad + kk * (16 * 128 / 16), bd, id_pv, (!begin || kk) ? 1u : 0u);
-          }
-          tc_commit(&sh.empty[pv_slot]);
-          tc_commit(&sh.empty[pv_slot + 1]);
-          pv_slot = pv_slot + 2 == NST ? 0 : pv_slot + 2;
-        }
-        tc_commit(&sh.pv_done);
-      };
-      if (ahead && chunks > 0) scores();
-      for (long long k = 0; k < chunks; ++k) {
-        if (!ahead)
-          scores();
-        else if (k + 1 < chunks)
-          scores();
-        outputs(k);
+        q_phase ^= 1;
       }
-      // every product of this CTA is done before TMEM is released
-      tc_commit(&sh.last);
-      mbar_wait(&sh.last, 0, DSV4_DEVERR_TIMEOUT_MMA);
+      i = 0;
+      if (++g >= a.groups) {
+        g = 0;
+        ++t;
+        sp = sp_next;
+      }
     }
+    while (ok && k_pv < k_qk) {
+      const uint32_t due = k_pv;
+      pv_blocking();
+      if (ok && k_pv == due) issue_pv();
+    }
+    // every product of this CTA is done before TMEM is released
+    if (el) tc_commit(&sh.last);
+    mbar_wait(&sh.last, 0, DSV4_DEVERR_TIMEOUT_MMA);
     __syncwarp();
   } else {
     // ----------------------------------------------------------- softmax
     const int st = tid - 64;                  // 0 .. 255
-    const int q4 = warp & 3;                  // TMEM lane quarter
-    const int h0 = warp < 6 ? 0 : HPT;        // warps 2-5 the first half of the heads, 6-9 the second
-    const int row = q4 * 32 + lane;           // cache row of the chunk; channel of a 128-channel tile
+    const int wi = warp - 2;                  // 0 .. 7
+    const int q4 = warp & 3, half = wi >> 2;  // TMEM lane quarter; key half, then head half
+    const int ha = 16 * q4 + (lane >> 2);     // this thread's heads: ha and ha + 8
+    const bool active = 16 * q4 < N;          // quarters past N hold no heads
+    const int c0 = 32 * half + 2 * (lane & 3);  // its keys: c0 + 8c and c0 + 8c + 1, c = 0 .. 3
+    const int row = q4 * 32 + lane, h0 = half * HPT;  // output: channel of a 128-channel block, heads
     const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
+    const float scale2 = a.scale * kLog2e;
     T* out = static_cast<T*>(a.out);
 
     // rows that see nothing
-    for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
-      if (pa_row(a, t).n) continue;
-      uint4* o = reinterpret_cast<uint4*>(out + (size_t)t * a.H * a.D);
+    for (int z = blockIdx.x; z < a.T; z += gridDim.x) {
+      if (pa_row(a, pa_index(a, z)).n) continue;
+      uint4* o = reinterpret_cast<uint4*>(out + (size_t)z * a.H * a.D);
       for (int u = st; u < a.H * a.D / 8; u += kPaSoft) o[u] = make_uint4(0, 0, 0, 0);
     }
 
-    long long left = sh.left;
-    int t = sh.t0, g = sh.g0, i = sh.i0;
-    long long k = 0;    // chunks so far
-    int slot = 0;       // ring position of this chunk's first tile
+    uint32_t k = 0;     // chunks so far
+    int slot = 0;       // ring position of this chunk's first stage
     while (left > 0 && t < a.T) {
-      const PaRow r = pa_row(a, t);
+      const PaRow r = pa_row(a, sp);
+      const int2 sp_next = pa_index(a, t + 1);
       const int i_begin = i, i1 = (int)min((long long)r.n, i + left);
       if (i < i1) {
         const int* pages = a.table + (long long)r.s * a.max_pages;
-        float l_run[HPT];
-#pragma unroll
-        for (int x = 0; x < HPT; ++x) l_run[x] = 0.f;
-        if (st < N) sh.m[st] = kPaNoMax;
-        soft_sync();
         left -= i1 - i;
-        auto page_at = [&](int c) -> int {
-          const int key = pa_key0(r, c) + row;
-          if (key > r.p || (key < r.w_lo && key >= r.f)) return -1;
-          const int p = __ldg(pages + key / a.page_size);
-          if (p < 0 || p >= a.n_pages) {
-            record_error(DSV4_DEVERR_BAD_CACHE_INDEX);
-            return -1;
-          }
-          return p;
+        // Whether key slot x of the chunk from box b on is visible, and its page there.
+        auto seen = [&](int b, int x) -> bool {
+          b += x >> a.box_log;
+          if (b >= i1) return false;
+          const int key = pa_box_key(a, r, b) + (x & ((1 << a.box_log) - 1));
+          if (key > r.p || (key < r.w_lo && key >= r.f)) return false;
+          const int p = __ldg(pages + (key >> a.page_log));
+          if (p >= 0 && p < a.n_pages) return true;
+          record_error(DSV4_DEVERR_BAD_CACHE_INDEX);
+          return false;
         };
-        int page_next = page_at(i);
-        for (; i < i1; ++i, ++k) {
-          const bool valid = page_next >= 0;
-          if (i + 1 < i1) page_next = page_at(i + 1);
-          const int b = (int)(k & 1);
-          pa_wait(sh, &sh.s_full[b], (uint32_t)(k >> 1) & 1, DSV4_DEVERR_TIMEOUT_EPILOGUE);
+        float m_a = kPaNoMax, m_b = kPaNoMax, l_a = 0.f, l_b = 0.f;
+        bool see0 = seen(i, lane), see1 = seen(i, lane + 32);
+        for (; i < i1; i += nsub, ++k) {
+          const uint32_t lo = __ballot_sync(0xffffffffu, see0), hi = __ballot_sync(0xffffffffu, see1);
+          if (i + nsub < i1) {
+            see0 = seen(i + nsub, lane);
+            see1 = seen(i + nsub, lane + 32);
+          }
+          const uint32_t b = k & 1, u = (k >> 1) & 1;
+          pa_wait(sh, &sh.s_full[b], u, DSV4_DEVERR_TIMEOUT_EPILOGUE);
           tc_fence_after();
-          float z[HPT];
-          tmem_ldn<HPT>(t_s + 64 * b + lane_base + h0, z);
-          tc_fence_before();
+          float z[16];
+          float top_a = -INFINITY, top_b = -INFINITY;
+          if (active) {
+            tmem_ld_16x32(t_s + 64 * b + 32 * half + lane_base, z);
+            tc_fence_before();
+#pragma unroll
+            for (int x = 0; x < 16; ++x) z[x] *= scale2;
+            const uint32_t mask = (half ? hi : lo) >> (2 * (lane & 3));
+            if (mask != (0xffffffffu >> (2 * (lane & 3)))) {
+#pragma unroll
+              for (int x = 0; x < 16; ++x)
+                if (!(mask >> (8 * (x >> 2) + (x & 1)) & 1)) z[x] = -INFINITY;
+            }
+#pragma unroll
+            for (int x = 0; x < 16; x += 4) {
+              top_a = fmaxf(top_a, fmaxf(z[x], z[x + 1]));
+              top_b = fmaxf(top_b, fmaxf(z[x + 2], z[x + 3]));
+            }
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.s_free[b]);
-          float over = -INFINITY;  // how far the scores exceed the running max
-          if (valid) {
-#pragma unroll
-            for (int x = 0; x < HPT; x += 4) {
-              const float4 m4 = *reinterpret_cast<const float4*>(&sh.m[h0 + x]);
-              over = fmaxf(over, fmaxf(fmaf(z[x], scale2, -m4.x), fmaf(z[x + 1], scale2, -m4.y)));
-              over = fmaxf(over, fmaxf(fmaf(z[x + 2], scale2, -m4.z), fmaf(z[x + 3], scale2, -m4.w)));
-            }
-          }
-          if (!valid) {
-            // whatever lies in the hidden row must not reach the output product (0 x NaN):
-            // this thread clears its half of the row's channels
-            int s = slot + (h0 ? KT / 2 : 0);
-            for (int kt = 0; kt < KT / 2; ++kt, ++s) {
-              uint4* dst = reinterpret_cast<uint4*>(ring + (s >= NST ? s - NST : s) * kPaTile + row * 128);
-#pragma unroll
-              for (int x = 0; x < 8; ++x) dst[x] = make_uint4(0, 0, 0, 0);
-            }
-          }
-          // the previous chunk's output product has read P and written O
-          if (k > 0) pa_wait(sh, &sh.pv_done, (uint32_t)(k - 1) & 1, DSV4_DEVERR_TIMEOUT_EPILOGUE);
-          if (soft_or(over > kPaRescaleLog2)) {
-            // raise every head's max to its largest score so far
-            tc_fence_after();
-            float v[HPT];
-#pragma unroll
-            for (int x = 0; x < HPT; ++x) v[x] = valid ? z[x] * scale2 : -INFINITY;
-            const float top = warp_reduce_n<HPT, false>(v, lane);
-            if (lane < HPT) sh.red[q4 * 64 + h0 + lane] = top;
-            soft_sync();
-            if (st < N) {
-              const float cm = fmaxf(fmaxf(sh.red[st], sh.red[64 + st]), fmaxf(sh.red[128 + st], sh.red[192 + st]));
-              const float mo = sh.m[st], mn = fmaxf(mo, cm);
-              sh.f[st] = ex2(mo - mn);
-              sh.m[st] = mn;
+          if (soft_or(top_a > m_a + kPaRescaleLog2 || top_b > m_b + kPaRescaleLog2)) {
+            // raise every head's max to its largest score so far, over both key halves
+            if (active) {
+              top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, 1));
+              top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 1));
+              top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, 2));
+              top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, 2));
+              if ((lane & 3) == 0) {
+                sh.red[64 * half + ha] = top_a;
+                sh.red[64 * half + ha + 8] = top_b;
+              }
             }
             soft_sync();
-#pragma unroll
-            for (int x = 0; x < HPT; ++x) l_run[x] *= sh.f[h0 + x];
+            if (active) {
+              const float n_a = fmaxf(m_a, fmaxf(sh.red[ha], sh.red[64 + ha]));
+              const float n_b = fmaxf(m_b, fmaxf(sh.red[ha + 8], sh.red[64 + ha + 8]));
+              const float f_a = ex2(m_a - n_a), f_b = ex2(m_b - n_b);
+              m_a = n_a;
+              m_b = n_b;
+              l_a *= f_a;
+              l_b *= f_b;
+              if ((lane & 3) == 0 && half == 0) {
+                sh.f[ha] = f_a;
+                sh.f[ha + 8] = f_b;
+              }
+            }
             if (i > i_begin) {
+              pa_wait(sh, &sh.pv_done[b ^ 1], ((k - 1) >> 1) & 1, DSV4_DEVERR_TIMEOUT_EPILOGUE);
+              soft_sync();
+              tc_fence_after();
               for (int dt = 0; dt < DT; ++dt) {
                 float o[HPT];
                 tmem_ldn<HPT>(t_o + N * dt + h0 + lane_base, o);
@@ -587,56 +663,68 @@ __global__ void __launch_bounds__(kPaThreads, 1)
               }
               tmem_wait_st();
             }
+            soft_sync();  // sh.red and sh.f are read before they are written again
           }
-          // weights, rounded to the cache's type as the product takes them; the sum adds
-          // them unrounded (their rounding errors average out over the keys)
-          if constexpr (N == 64) {
-            // P[j][h], heads contiguous: 128-byte rows, 128-byte swizzle (MN-major operand)
-            uint8_t* prow = sP + row * 128;
-#pragma unroll
-            for (int x = 0; x < HPT; x += 8) {
-              Pack<T, 8> w;
-#pragma unroll
-              for (int y = 0; y < 8; y += 4) {
-                const float4 m4 = *reinterpret_cast<const float4*>(&sh.m[h0 + x + y]);
-                const float mm[4] = {m4.x, m4.y, m4.z, m4.w};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  const float e = valid ? ex2(fmaf(z[x + y + c], scale2, -mm[c])) : 0.f;
-                  l_run[x + y + c] += e;
-                  w.v[y + c] = from_f32<T>(e);
-                }
+          // the output product of two chunks ago has read this buffer of P
+          if (k > 1) pa_wait(sh, &sh.pv_done[b], u ^ 1, DSV4_DEVERR_TIMEOUT_EPILOGUE);
+          if ((lo & hi) != 0xffffffffu) {
+            // whatever lies in a hidden row must not reach the output product (0 x NaN)
+            for (int x = wi; x < kPaChunk; x += 8) {
+              if ((x < 32 ? lo >> x : hi >> (x - 32)) & 1) continue;
+              for (int y = lane; y < 16 * DT; y += 32) {
+                int s = slot + (y >> 4);
+                if (s >= NST) s -= NST;
+                *reinterpret_cast<uint4*>(ring + s * kPaStage + ((y >> 3) & 1) * kPaTile + x * 128 + (y & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
               }
-              store_pack<T, 8>(reinterpret_cast<T*>(prow + ((((h0 + x) >> 3) ^ (row & 7)) << 4)), w);
             }
-          } else {
-            // P[h][j], keys contiguous (K-major operand): 16 or 8 heads per thread
+          }
+          if (active) {
+            // weights, rounded to the cache's type as the product takes them; the sum adds
+            // them unrounded (their rounding errors average out over the keys)
+            uint8_t* p0 = sP + b * (N * 128) + ha * 128 + 4 * (lane & 3);
 #pragma unroll
-            for (int x = 0; x < HPT; ++x) {
-              const float e = valid ? ex2(fmaf(z[x], scale2, -sh.m[h0 + x])) : 0.f;
-              l_run[x] += e;
-              *reinterpret_cast<T*>(sP + sw128_offset(N, h0 + x, row)) = from_f32<T>(e);
+            for (int c = 0; c < 4; ++c) {
+              const float e0 = ex2(z[4 * c] - m_a), e1 = ex2(z[4 * c + 1] - m_a);
+              const float e2 = ex2(z[4 * c + 2] - m_b), e3 = ex2(z[4 * c + 3] - m_b);
+              l_a += e0 + e1;
+              l_b += e2 + e3;
+              const int unit = ((4 * half + c) ^ (ha & 7)) << 4;  // rows ha and ha + 8 swizzle alike
+              *reinterpret_cast<uint32_t*>(p0 + unit) = pack2<T>(e0, e1);
+              *reinterpret_cast<uint32_t*>(p0 + 8 * 128 + unit) = pack2<T>(e2, e3);
             }
           }
           fence_proxy_async_shared();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.p_ready);
-          slot += KT;
+          if (lane == 0) mbar_arrive(&sh.p_ready[b]);
+          slot += DT;
           if (slot >= NST) slot -= NST;
         }
         // ---- the piece's output: O^T columns times a factor per head
-        pa_wait(sh, &sh.pv_done, (uint32_t)(k - 1) & 1, DSV4_DEVERR_TIMEOUT_EPILOGUE);
+        if (active) {
+#pragma unroll
+          for (int o = 1; o < 4; o <<= 1) {
+            l_a += __shfl_xor_sync(0xffffffffu, l_a, o);
+            l_b += __shfl_xor_sync(0xffffffffu, l_b, o);
+          }
+          if ((lane & 3) == 0) {
+            sh.red[64 * half + ha] = l_a;
+            sh.red[64 * half + ha + 8] = l_b;
+            if (half == 0) {
+              sh.m[ha] = m_a;
+              sh.m[ha + 8] = m_b;
+            }
+          }
+        }
+        pa_wait(sh, &sh.pv_done[(k - 1) & 1], ((k - 1) >> 1) & 1, DSV4_DEVERR_TIMEOUT_EPILOGUE);
         tc_fence_after();
-        const float sum = warp_reduce_n<HPT, true>(l_run, lane);
-        if (lane < HPT) sh.red[q4 * 64 + h0 + lane] = sum;
         soft_sync();
         const bool whole = i_begin == 0 && i1 == r.n;
         const size_t piece = (size_t)blockIdx.x * 2 + (i_begin == 0);
         const int heads = min(N, a.H - 64 * g);
         if (st < N) {
-          const float l = (sh.red[st] + sh.red[64 + st]) + (sh.red[128 + st] + sh.red[192 + st]);
-          const float m = sh.m[st];
+          const float l = sh.red[st] + sh.red[64 + st], m = sh.m[st];
           if (whole) {
             const float sk = a.sink && st < heads ? __ldg(a.sink + 64 * g + st) * kLog2e : -INFINITY;
             const float mx = fmaxf(m, sk);
@@ -670,6 +758,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       if (++g >= a.groups) {
         g = 0;
         ++t;
+        sp = sp_next;
       }
     }
   }
@@ -703,7 +792,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaA
   int n_rows = 0;  // in border order, so that every CTA has the same list
   for (int base = 1; base < n_plan; base += kJoinThreads) {
     const int c = base + threadIdx.x;
-    int4 pl = make_int4(-1, 0, 0, 0);  // row, group, chunks before the border, chunks of the row
+    int4 pl = make_int4(-1, 0, 0, 0);  // row, group, boxes before the border, boxes of the row
     if (c < n_plan) pl = a.plan[c];
     const bool on = pl.x >= 0 && pl.z > 0 && pl.z <= share;
     const unsigned vote = __ballot_sync(0xffffffffu, on);
@@ -797,10 +886,9 @@ static PaShape pa_shape(int T, int H, int D, long long max_keys, int num_sms) {
   s.N = H > 32 ? 64 : H > 16 ? 32 : 16;
   s.groups = (H + 63) / 64;
   const int fixed = 1024 + (D / 64) * s.N * 128 + 2 * s.N * 128 + kPaCtrl;
-  s.stages = (kPaSmemMax - fixed) / kPaTile;
+  s.stages = (kPaSmemMax - fixed) / kPaStage;
   if (s.stages > kPaMaxStages) s.stages = kPaMaxStages;
-  s.stages &= ~1;  // two tiles of one 128-channel output block lie side by side
-  s.smem = (size_t)fixed + (size_t)s.stages * kPaTile;
+  s.smem = (size_t)fixed + (size_t)s.stages * kPaStage;
   const long long most = (long long)T * s.groups * ((max_keys + kPaChunk - 1) / kPaChunk);
   if (num_sms > kPaMaxGrid) num_sms = kPaMaxGrid;
   s.grid = (int)(most < num_sms ? (most < 1 ? 1 : most) : num_sms);
@@ -874,12 +962,13 @@ int launch_paged_attn(const void* q, bool fp16, int T, int H, int D, long long q
   a.n_seqs = n_seqs;
   a.max_pages = max_pages;
   a.n_pages = n_pages;
-  a.page_size = page_size;
+  while (1 << a.page_log < page_size) ++a.page_log;
+  a.box_log = a.page_log < 6 ? a.page_log : 6;
   a.idx64 = idx64;
   a.window = window;
   a.first = first;
   a.stages = s.stages;
-  a.min_share = 1;
+  a.min_share = kPaChunk >> a.box_log;  // a chunk
   a.scale = scale;
   if (fp16) {
     if (s.N == 64) return launch_paged_attn_t<__half, 64>(s, qm, kvm, a, st);
