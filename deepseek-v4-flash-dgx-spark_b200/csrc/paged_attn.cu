@@ -32,13 +32,13 @@
 // lengths of each replay.  A row that crosses a border leaves fp32 partials (max,
 // sum, O) that paged_attn_join_kernel merges; every CTA has at most two such pieces.
 //
-// Warp roles (320 threads): warp 0 loads Q and the pages by TMA into a ring of
-// stages (64 keys x 128 channels, 16 KB), warp 1 issues the products, warps 2-9 do
+// Warp roles (352 threads): warp 0 loads Q and the pages by TMA into a ring of
+// stages (64 keys x 128 channels, 16 KB), warp 1 issues the score products as the
+// stages arrive, up to a chunk ahead of warp 2, which issues the output products
+// when their weights are there and gives the stages back one by one.  Warps 3-10 do
 // the softmax: warp w takes the heads of TMEM quarter w % 4 and half of the chunk's
-// keys, and at the end the channels of that quarter and half of the heads.  The
-// scores of chunk k + 1 are issued as its stages arrive; the output product of
-// chunk k goes in between as soon as its weights are there, and gives its stages
-// back one by one.
+// keys, and at the end the channels of that quarter and half of the heads.  (One
+// warp for both products spends 4000 cycles a chunk on issuing and polling.)
 #include <limits.h>
 
 #include <type_traits>
@@ -48,8 +48,8 @@
 namespace dsv4 {
 
 constexpr int kPaChunk = 64;                      // keys per chunk
-constexpr int kPaThreads = 320;
-constexpr int kPaSoft = 256;                      // softmax threads: warps 2-9
+constexpr int kPaThreads = 352;
+constexpr int kPaSoft = 256;                      // softmax threads: warps 3-10
 constexpr int kPaTile = kPaChunk * 128;           // 8 KB: 64 keys x 64 channels, 128-byte swizzled
 constexpr int kPaStage = 2 * kPaTile;             // 16 KB: 64 keys x 128 channels
 constexpr int kPaMaxStages = 12;
@@ -111,7 +111,7 @@ __device__ __forceinline__ int pa_box_key(const PaArgs& a, const PaRow& r, int b
 
 struct PaShared {
   uint64_t full[kPaMaxStages], empty[kPaMaxStages];
-  uint64_t q_full[4], q_empty, s_full[2], s_free[2], p_ready[2], pv_done[2], last;
+  uint64_t q_full[4], q_empty, s_full[2], s_free[2], p_ready[2], pv_done[2], last[2];
   uint32_t tmem;
   int abort;
   int t0, g0, i0;           // this CTA's first row, head group and box
@@ -121,18 +121,6 @@ struct PaShared {
   float m[64], f[64];       // max, factor per head
 };
 static_assert(sizeof(PaShared) <= kPaCtrl, "control block too small");
-
-__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 
 __device__ __forceinline__ bool pa_aborted(PaShared& sh) { return *reinterpret_cast<volatile int*>(&sh.abort) != 0; }
 
@@ -285,7 +273,8 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       mbar_init(&sh.p_ready[i], kPaSoft / 32);
       mbar_init(&sh.pv_done[i], 1);
     }
-    mbar_init(&sh.last, 1);
+    mbar_init(&sh.last[0], 1);
+    mbar_init(&sh.last[1], 1);
     fence_barrier_init();
     sh.abort = 0;
     sh.left = 0;
@@ -440,98 +429,59 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       for (int k = 0; k < DT; ++k) mbar_wait(&sh.q_full[k], q_phase ^ 1, DSV4_DEVERR_TIMEOUT_PRODUCER);
     __syncwarp();
   } else if (warp == 1) {
-    // ---------------------------------------------------------- products
+    // ---------------------------------------------------- score products
     // All lanes run the loops, so that descriptors stay in uniform registers; one issues.
     const bool el = elect_one();
-    constexpr uint32_t id_qk = pa_idesc<T>(64, kPaChunk, 0), id_pv = pa_idesc<T>(128, N, 1);
+    constexpr uint32_t id = pa_idesc<T>(64, kPaChunk, 0);
     // descriptors of the first tile; an address moves the low field by bytes / 16
     const uint64_t dq = sdesc_k_sw128(smem_u32(sQ)), dk = sdesc_k_sw128(smem_u32(ring));
-    const uint64_t dm = sdesc_mn_sw128(smem_u32(ring), kPaTile), dp = sdesc_k_sw128(smem_u32(sP));
     bool ok = true;
-    uint32_t k_qk = 0, k_pv = 0;  // chunks whose products are issued
-    uint32_t begins = 0;          // bit k % 32: chunk k begins a piece, its output starts anew
-    int slot = 0, pv_slot = 0;
+    uint32_t k = 0;  // chunks so far
+    int slot = 0;
     uint32_t phase = 0, q_phase = 0;
-
-    auto issue_pv = [&]() {
-      tc_fence_after();
-      const uint32_t b = k_pv & 1;
-      const uint32_t begin = (begins >> (k_pv & 31)) & 1;
-      for (int dt = 0; dt < DT; ++dt) {
-        if (el) {
-          const uint64_t ad = dm + pv_slot * (kPaStage / 16), bd = dp + b * (N * 128 / 16);
-#pragma unroll
-          for (int kk = 0; kk < kPaChunk / 16; ++kk)
-            tc_mma_f16(t_o + N * dt, ad + kk * (16 * 128 / 16), bd + 2 * kk, id_pv, (begin && kk == 0) ? 0u : 1u);
-          tc_commit(&sh.empty[pv_slot]);
-        }
-        if (++pv_slot == NST) pv_slot = 0;
-      }
-      if (el) tc_commit(&sh.pv_done[b]);
-      ++k_pv;
-    };
-    // Wait for a barrier; an output product whose weights get ready meanwhile is issued.
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      uint64_t t0 = 0;
-      for (uint32_t n = 1; ok; ++n) {
-        if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) break;
-        if (k_pv < k_qk && __all_sync(0xffffffffu, mbar_test_wait(&sh.p_ready[k_pv & 1], (k_pv >> 1) & 1))) issue_pv();
-        if ((n & 255) == 0) {
-          const uint64_t now = globaltimer();
-          if (t0 == 0) t0 = now;
-          if (now - t0 > kWaitTimeoutNs && lane == 0) {
-            record_error(DSV4_DEVERR_TIMEOUT_MMA);
-            *reinterpret_cast<volatile int*>(&sh.abort) = 1;
-          }
-          __syncwarp();
-          ok = !__any_sync(0xffffffffu, pa_aborted(sh));
-        }
-      }
-    };
-    auto pv_blocking = [&]() {
-      wait(&sh.p_ready[k_pv & 1], (k_pv >> 1) & 1);
-    };
-
     while (left > 0 && ok && t < a.T) {
-      const int n = __shfl_sync(0xffffffffu, pa_row(a, sp).n, 0);
+      const int n = pa_row(a, sp).n;
       const int2 sp_next = pa_index(a, t + 1);
       const int i1 = (int)min((long long)n, i + left);
       if (i < i1) {
         left -= i1 - i;
         bool begin = true;
-        for (; i < i1 && ok; i += nsub) {
-          const uint32_t b = k_qk & 1;
-          wait(&sh.s_free[b], ((k_qk >> 1) & 1) ^ 1);
-          for (int dt = 0; dt < DT && ok; ++dt) {
-            if (begin) wait(&sh.q_full[dt], q_phase);
-            wait(&sh.full[slot], phase);
+        for (; i < i1 && ok; i += nsub, ++k) {
+          const uint32_t b = __shfl_sync(0xffffffffu, k & 1, 0);
+          const uint32_t d = __shfl_sync(0xffffffffu, t_s, 0) + 64 * b;
+          const int slot0 = __shfl_sync(0xffffffffu, slot, 0);
+          ok = pa_wait(sh, &sh.s_free[b], ((k >> 1) & 1) ^ 1, DSV4_DEVERR_TIMEOUT_MMA);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) {
+            if (dt >= DT) break;
+            if (begin) ok = ok && pa_wait(sh, &sh.q_full[dt], q_phase, DSV4_DEVERR_TIMEOUT_MMA);
+            int su = slot0 + dt;
+            uint32_t ph = phase;
+            if (su >= NST) {
+              su -= NST;
+              ph ^= 1;
+            }
+            ok = ok && pa_wait(sh, &sh.full[su], ph, DSV4_DEVERR_TIMEOUT_MMA);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             if (el) {
-              const uint64_t ad = dq + dt * (2 * N * 128 / 16), bd = dk + slot * (kPaStage / 16);
+              const uint64_t ad = dq + dt * (2 * N * 128 / 16), bd = dk + su * (kPaStage / 16);
 #pragma unroll
               for (int kk = 0; kk < 8; ++kk)
-                tc_mma_f16(t_s + 64 * b, ad + (kk >> 2) * (N * 128 / 16) + 2 * (kk & 3),
-                           bd + (kk >> 2) * (kPaTile / 16) + 2 * (kk & 3), id_qk, (dt || kk) ? 1u : 0u);
-            }
-            if (++slot == NST) {
-              slot = 0;
-              phase ^= 1;
+                tc_mma_f16(d, ad + (kk >> 2) * (N * 128 / 16) + 2 * (kk & 3),
+                           bd + (kk >> 2) * (kPaTile / 16) + 2 * (kk & 3), id, (dt || kk) ? 1u : 0u);
             }
           }
-          if (!ok) break;
-          if (el) {
+          if (ok && el) {
             tc_commit(&sh.s_full[b]);
             if (i + nsub >= i1) tc_commit(&sh.q_empty);  // the piece's last use of Q
           }
-          begins = begin ? begins | (1u << (k_qk & 31)) : begins & ~(1u << (k_qk & 31));
           begin = false;
-          ++k_qk;
-          // at most one chunk's output waits while the next scores are issued
-          if (k_qk - k_pv > 1) {
-            const uint32_t due = k_pv;
-            pv_blocking();
-            if (ok && k_pv == due) issue_pv();
+          slot += DT;
+          if (slot >= NST) {
+            slot -= NST;
+            phase ^= 1;
           }
         }
         q_phase ^= 1;
@@ -543,19 +493,65 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         sp = sp_next;
       }
     }
-    while (ok && k_pv < k_qk) {
-      const uint32_t due = k_pv;
-      pv_blocking();
-      if (ok && k_pv == due) issue_pv();
+    // every product of this warp is done before TMEM is released
+    if (el) tc_commit(&sh.last[0]);
+    mbar_wait(&sh.last[0], 0, DSV4_DEVERR_TIMEOUT_MMA);
+    __syncwarp();
+  } else if (warp == 2) {
+    // --------------------------------------------------- output products
+    const bool el = elect_one();
+    constexpr uint32_t id = pa_idesc<T>(128, N, 1);
+    const uint64_t dm = sdesc_mn_sw128(smem_u32(ring), kPaTile), dp = sdesc_k_sw128(smem_u32(sP));
+    bool ok = true;
+    uint32_t k = 0;
+    int slot = 0;
+    while (left > 0 && ok && t < a.T) {
+      const int n = pa_row(a, sp).n;
+      const int2 sp_next = pa_index(a, t + 1);
+      const int i1 = (int)min((long long)n, i + left);
+      if (i < i1) {
+        left -= i1 - i;
+        bool begin = true;  // the piece's output starts anew
+        for (; i < i1 && ok; i += nsub, ++k) {
+          const uint32_t b = __shfl_sync(0xffffffffu, k & 1, 0);
+          const uint32_t d = __shfl_sync(0xffffffffu, t_o, 0);
+          const int slot0 = __shfl_sync(0xffffffffu, slot, 0);
+          const uint32_t more = __shfl_sync(0xffffffffu, begin ? 0 : 1, 0);
+          ok = __all_sync(0xffffffffu, pa_wait(sh, &sh.p_ready[b], (k >> 1) & 1, DSV4_DEVERR_TIMEOUT_MMA));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) {
+            if (dt >= DT) break;
+            const int su = slot0 + dt >= NST ? slot0 + dt - NST : slot0 + dt;
+            if (el) {
+              const uint64_t ad = dm + su * (kPaStage / 16), bd = dp + b * (N * 128 / 16);
+#pragma unroll
+              for (int kk = 0; kk < kPaChunk / 16; ++kk)
+                tc_mma_f16(d + N * dt, ad + kk * (16 * 128 / 16), bd + 2 * kk, id, kk ? 1u : more);
+              tc_commit(&sh.empty[su]);
+            }
+          }
+          if (el) tc_commit(&sh.pv_done[b]);
+          begin = false;
+          slot += DT;
+          if (slot >= NST) slot -= NST;
+        }
+      }
+      i = 0;
+      if (++g >= a.groups) {
+        g = 0;
+        ++t;
+        sp = sp_next;
+      }
     }
-    // every product of this CTA is done before TMEM is released
-    if (el) tc_commit(&sh.last);
-    mbar_wait(&sh.last, 0, DSV4_DEVERR_TIMEOUT_MMA);
+    if (el) tc_commit(&sh.last[1]);
+    mbar_wait(&sh.last[1], 0, DSV4_DEVERR_TIMEOUT_MMA);
     __syncwarp();
   } else {
     // ----------------------------------------------------------- softmax
-    const int st = tid - 64;                  // 0 .. 255
-    const int wi = warp - 2;                  // 0 .. 7
+    const int st = tid - 96;                  // 0 .. 255
+    const int wi = warp - 3;                  // 0 .. 7
     const int q4 = warp & 3, half = wi >> 2;  // TMEM lane quarter; key half, then head half
     const int ha = 16 * q4 + (lane >> 2);     // this thread's heads: ha and ha + 8
     const bool active = 16 * q4 < N;          // quarters past N hold no heads
