@@ -1066,7 +1066,7 @@ int dsv4_rotary(const void* x, void* y, int dtype, const void* positions, int po
                 const long long* x_strides, const long long* y_strides, void* stream) {
   if (B < 0 || S < 0 || H < 0 || D <= 0 || !rotary_shape_ok(D, rot, offset)) return DSV4_ERR_ARG;
   if (dtype < DSV4_DTYPE_BF16 || dtype > DSV4_DTYPE_FP32) return DSV4_ERR_UNSUPPORTED;
-  if (rot > kRotMax || D > (1 << 20)) return DSV4_ERR_UNSUPPORTED;
+  if (rot > kRotMax || D > kRotMaxDim) return DSV4_ERR_UNSUPPORTED;
   if (B == 0 || S == 0 || H == 0) return DSV4_OK;
   if (!x || !y || !x_strides || !y_strides || (rot && (!positions || !freqs))) return DSV4_ERR_ARG;
   for (int i = 0; i < 3; ++i)

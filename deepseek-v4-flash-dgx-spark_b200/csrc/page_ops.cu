@@ -107,19 +107,6 @@ __device__ __forceinline__ int pages_of(int len, int page_size) {
   return len <= 0 ? 0 : (len - 1) / page_size + 1;
 }
 
-// start[i] <= k < start[i + 1] over n entries (start[n] is the total).
-__device__ __forceinline__ int find_entry(const int* start, int n, int k) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (start[mid] <= k)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
-}
-
 // Workspace: owner [n_seqs], start [n + 1], picked [n_pages].
 __global__ void __launch_bounds__(kPlanThreads) cache_reserve_kernel(const PageState st, const int* seqs,
                                                                      const int* new_lens, int n, int* ws) {
@@ -159,10 +146,19 @@ __global__ void __launch_bounds__(kPlanThreads) cache_reserve_kernel(const PageS
     if (threadIdx.x == 0) record_error(DSV4_DEVERR_NO_PAGES);
     return;
   }
-  for (int k = threadIdx.x; k < total; k += kPlanThreads) {
-    const int i = find_entry(start, n, k), s = seqs[i];
-    st.table[(long long)s * st.max_pages + pages_of(st.lens[s], st.page_size) + (k - start[i])] = picked[k];
-    st.refs[picked[k]] = 1;
+  // a warp per entry, or several where the entries are few
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int share = n < kPlanWarps ? kPlanWarps / n : 1;
+  for (int e = w; e < n * share; e += kPlanWarps) {
+    const int i = e / share, from = start[i], to = start[i + 1];
+    if (from == to) continue;
+    const int s = seqs[i];
+    int* row = st.table + (long long)s * st.max_pages + pages_of(st.lens[s], st.page_size) - from;
+    for (int k = from + (e % share) * 32 + lane; k < to; k += 32 * share) {
+      const int p = picked[k];
+      row[k] = p;
+      st.refs[p] = 1;
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kPlanThreads) {

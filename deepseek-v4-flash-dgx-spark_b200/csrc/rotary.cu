@@ -94,42 +94,61 @@ __host__ __device__ __forceinline__ int head_units(const RotaryShape& r) {
   return rotary_units<V>(r) + (r.D - r.rot) / V;
 }
 
-// One unit of one head: x, y are the head's channel 0; cs the pairs' cosines and sines.
-template <typename T, int V>
-__device__ __forceinline__ void rotary_unit(const T* x, T* y, int u, int n_rot, const RotaryShape& r, const float2* cs) {
-  using P = Pack<T, V>;
-  if (u >= n_rot) {  // a pass-through pack, before or behind the rotated channels
-    int c = (u - n_rot) * V;
-    if (c >= r.offset) c += r.rot;
-    store_pack<T, V>(y + c, load_pack<T, V>(x + c));
-    return;
-  }
-  if (r.interleaved && V > 1) {
-    const int c = r.offset + u * V;
-    P p = load_pack<T, V>(x + c);
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      const float2 t = cs[u * (V / 2) + i];
-      const float a = to_f32(p.v[2 * i]), b = to_f32(p.v[2 * i + 1]);
-      p.v[2 * i] = from_f32<T>(a * t.x - b * t.y);
-      p.v[2 * i + 1] = from_f32<T>(b * t.x + a * t.y);
+// One unit of one head, loaded, turned and stored in three steps so that a thread has
+// the loads of several units in flight (x and y may be the same memory, so the
+// compiler cannot move a load above a store).  x, y are the head's channel 0.
+template <typename T, int V, bool kInter>
+struct RotaryUnit {
+  static constexpr bool kTwo = V == 1 || !kInter;  // a rotating unit has two packs
+  Pack<T, V> p, q;
+  int ca, cb;
+
+  __device__ __forceinline__ void load(const T* x, int u, int n_rot, const RotaryShape& r) {
+    if (u >= n_rot) {  // a pass-through pack, before or behind the rotated channels
+      ca = (u - n_rot) * V;
+      if (ca >= r.offset) ca += r.rot;
+    } else if (kTwo) {
+      ca = r.offset + (kInter ? 2 * u : u * V);
+      cb = kInter ? ca + 1 : ca + r.rot / 2;
+      q = load_pack<T, V>(x + cb);
+    } else {
+      ca = r.offset + u * V;
     }
-    store_pack<T, V>(y + c, p);
-    return;
+    p = load_pack<T, V>(x + ca);
   }
-  const int ca = r.offset + (r.interleaved ? 2 * u : u * V);
-  const int cb = r.interleaved ? ca + 1 : ca + r.rot / 2;
-  P p = load_pack<T, V>(x + ca), q = load_pack<T, V>(x + cb);
+
+  __device__ __forceinline__ void turn_and_store(T* y, int u, int n_rot, const float2* cs) {
+    if (u < n_rot) {
+      if constexpr (kTwo) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float2 t = cs[u * V + i];
-    const float a = to_f32(p.v[i]), b = to_f32(q.v[i]);
-    p.v[i] = from_f32<T>(a * t.x - b * t.y);
-    q.v[i] = from_f32<T>(b * t.x + a * t.y);
+        for (int i = 0; i < V; ++i) {
+          const float2 t = cs[u * V + i];
+          const float a = to_f32(p.v[i]), b = to_f32(q.v[i]);
+          p.v[i] = from_f32<T>(a * t.x - b * t.y);
+          q.v[i] = from_f32<T>(b * t.x + a * t.y);
+        }
+        store_pack<T, V>(y + cb, q);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          const float2 t = cs[u * (V / 2) + i];
+          const float a = to_f32(p.v[2 * i]), b = to_f32(p.v[2 * i + 1]);
+          p.v[2 * i] = from_f32<T>(a * t.x - b * t.y);
+          p.v[2 * i + 1] = from_f32<T>(b * t.x + a * t.y);
+        }
+      }
+    }
+    store_pack<T, V>(y + ca, p);
   }
-  store_pack<T, V>(y + ca, p);
-  store_pack<T, V>(y + cb, q);
-}
+};
+
+// n / d for n < 2^15 by a multiplication: ceil(2^32 / d) is off by less than d, which
+// moves the product by less than n d / 2^32 < 1 / 4 of a step while d < 2^15.
+struct FastDiv {
+  unsigned d, m;
+  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)__umulhi((unsigned)n, m); }
+};
+static FastDiv fast_div(int d) { return FastDiv{(unsigned)d, d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u}; }
 
 struct RotaryArgs {
   const void* x;
@@ -137,9 +156,9 @@ struct RotaryArgs {
   const void* positions;  // [B,S], int32 or int64
   const double* freqs;    // [rot / 2] radians per position
   long long xs[3], ys[3];  // strides of (b, s, h) in elements
-  int pos64, S, H;
-  long long tokens;
+  int pos64, S, H, tokens;
   int tile_tokens, tile_heads, head_tiles;  // one CTA: tile_tokens tokens x tile_heads heads
+  FastDiv by_head;                          // units per head
   int in_place, inverse;
   float amplitude;
   RotaryShape r;
@@ -147,19 +166,49 @@ struct RotaryArgs {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotMax = 4096;     // rotated channels per head
+constexpr int kRotMaxDim = 32760;  // channels per head (FastDiv)
 constexpr int kRotTable = 2048;   // cosine / sine pairs a CTA keeps (16 KB)
-constexpr int kRotUnits = 1024;   // units a CTA takes: four per thread
+constexpr int kRotBatch = 4;      // units per thread, their loads in flight together
+constexpr int kRotUnits = kRotThreads * kRotBatch;
+constexpr int kRotTokens = 64;    // tokens a CTA takes at most
 
-// One CTA takes a tile of tokens x heads: the tokens' cosines and sines go to
-// shared memory once, then every thread moves units of 16 bytes.
-template <typename T, int V>
+// One CTA takes a tile of tokens x heads.  Every thread has its first units on the
+// way before the tokens' cosines and sines are worked out for all heads.
+template <typename T, int V, bool kInter>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a) {
   __shared__ float2 cs[kRotTable];
-  const long long tok0 = (long long)(blockIdx.x / a.head_tiles) * a.tile_tokens;
+  const int tok0 = (int)(blockIdx.x / a.head_tiles) * a.tile_tokens;
   const int h0 = (blockIdx.x % a.head_tiles) * a.tile_heads;
-  const int n_tok = (int)min((long long)a.tile_tokens, a.tokens - tok0);
+  const int n_tok = min(a.tile_tokens, a.tokens - tok0);
   const int n_head = min(a.tile_heads, a.H - h0);
   const int pairs = a.r.rot / 2;
+  const int n_rot = rotary_units<V>(a.r);
+  const int per_head = (int)a.by_head.d, total = n_tok * n_head * per_head;
+  const T* x = static_cast<const T*>(a.x);
+  T* y = static_cast<T*>(a.y);
+
+  RotaryUnit<T, V, kInter> unit[kRotBatch];
+  int at[kRotBatch], un[kRotBatch];  // token within the tile, unit of the head
+  long long to[kRotBatch];           // where the head begins in y
+  auto load = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < kRotBatch; ++j) {
+      const int i = base + j * kRotThreads;
+      if (i >= total) continue;
+      const int th = a.by_head.div(i);  // token and head
+      un[j] = i - th * per_head;
+      at[j] = n_tok == 1 ? 0 : th / n_head;
+      const int h = h0 + th - at[j] * n_head;
+      int s = tok0 + at[j], b = 0;
+      if (a.S != a.tokens) {
+        b = s / a.S;
+        s -= b * a.S;
+      }
+      to[j] = b * a.ys[0] + s * a.ys[1] + h * a.ys[2];
+      unit[j].load(x + b * a.xs[0] + s * a.xs[1] + h * a.xs[2], un[j], n_rot, a.r);
+    }
+  };
+  load(threadIdx.x);
   for (int i = threadIdx.x; i < n_tok * pairs; i += kRotThreads) {
     const long long tok = tok0 + i / pairs;
     const long long pos = a.pos64 ? __ldg(static_cast<const long long*>(a.positions) + tok)
@@ -167,18 +216,11 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     cs[i] = rotary_cos_sin(pos, __ldg(a.freqs + i % pairs), a.amplitude, a.inverse != 0);
   }
   __syncthreads();
-  const int n_rot = rotary_units<V>(a.r);
-  const int per_head = a.in_place ? n_rot : head_units<V>(a.r);
-  const int per_tok = n_head * per_head;
-  const T* x = static_cast<const T*>(a.x);
-  T* y = static_cast<T*>(a.y);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n_tok * per_tok; i += kRotThreads) {
-    const int t = i / per_tok, j = i - t * per_tok;
-    const int h = j / per_head, u = j - h * per_head;
-    const long long tok = tok0 + t, b = tok / a.S, s = tok - b * a.S;
-    rotary_unit<T, V>(x + b * a.xs[0] + s * a.xs[1] + (long long)(h0 + h) * a.xs[2],
-                      y + b * a.ys[0] + s * a.ys[1] + (long long)(h0 + h) * a.ys[2], u, n_rot, a.r, cs + t * pairs);
+  for (int base = threadIdx.x; base < total; base += kRotUnits) {
+    if (base >= kRotUnits) load(base);
+#pragma unroll
+    for (int j = 0; j < kRotBatch; ++j)
+      if (base + j * kRotThreads < total) unit[j].turn_and_store(y + to[j], un[j], n_rot, cs + at[j] * pairs);
   }
 }
 
@@ -201,30 +243,42 @@ constexpr int kAppendPairs = 256;  // rot <= 512
 // One warp per row: its pairs' cosines and sines by its lanes, then units of 16
 // bytes from the row to its page.  Rows with a negative sequence or position are
 // padding and are skipped; others out of range, or on no page, are reported.
-template <typename T, int V>
+template <typename T, int V, bool kInter>
 __global__ void __launch_bounds__(32 * kAppendRows) cache_append_kernel(const AppendArgs a) {
   __shared__ float2 cs_all[kAppendRows][kAppendPairs];
+  constexpr int kBatch = 2;  // units in flight per lane: a row of 512 channels
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long t = (long long)blockIdx.x * kAppendRows + w;
   if (t >= a.T) return;
   const int s = a.seq_ids ? load_index(a.seq_ids, a.idx64, t) : (int)t;
   const int pos = load_index(a.positions, a.idx64, t);
+  const T* x = static_cast<const T*>(a.rows) + t * a.row_stride;
+  const int n_rot = rotary_units<V>(a.r), n = head_units<V>(a.r);
+  // the row's first units are on their way while the page is looked up
+  RotaryUnit<T, V, kInter> unit[kBatch];
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j)
+    if (lane + 32 * j < n) unit[j].load(x, lane + 32 * j, n_rot, a.r);
   if (s < 0 || pos < 0) return;
   const int slot = pos / a.page_size;
   int page = -1;
   if (s < a.n_seqs && slot < a.max_pages) page = __ldg(a.table + (long long)s * a.max_pages + slot);
+  float2* cs = cs_all[w];
+  for (int i = lane; i < a.r.rot / 2; i += 32) cs[i] = rotary_cos_sin(pos, __ldg(a.freqs + i), a.amplitude, false);
+  __syncwarp();
   if (page < 0 || page >= a.n_pages) {
     if (lane == 0) record_error(DSV4_DEVERR_BAD_CACHE_INDEX);
     return;
   }
-  float2* cs = cs_all[w];
-  for (int i = lane; i < a.r.rot / 2; i += 32) cs[i] = rotary_cos_sin(pos, __ldg(a.freqs + i), a.amplitude, false);
-  __syncwarp();
-  const T* x = static_cast<const T*>(a.rows) + t * a.row_stride;
-  T* y = static_cast<T*>(a.pages) + page * a.page_stride + (long long)(pos % a.page_size) * a.r.D;
-  const int n_rot = rotary_units<V>(a.r), n = head_units<V>(a.r);
-#pragma unroll 2
-  for (int u = lane; u < n; u += 32) rotary_unit<T, V>(x, y, u, n_rot, a.r, cs);
+  T* y = static_cast<T*>(a.pages) + page * a.page_stride + (long long)(pos - slot * a.page_size) * a.r.D;
+  for (int u = lane; u < n; u += 32 * kBatch) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (u > lane && u + 32 * j < n) unit[j].load(x, u + 32 * j, n_rot, a.r);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (u + 32 * j < n) unit[j].turn_and_store(y, u + 32 * j, n_rot, cs);
+  }
 }
 
 // Whether 16-byte packs of V elements never straddle a border.
@@ -245,16 +299,17 @@ static int launch_rotary_t(RotaryArgs a, cudaStream_t st) {
   if (a.tile_heads > a.H) a.tile_heads = a.H;
   a.head_tiles = (a.H + a.tile_heads - 1) / a.tile_heads;
   int tt = kRotUnits / (per_head * a.tile_heads);
-  const int by_table = a.r.rot ? kRotTable / (a.r.rot / 2) : 64;
+  const int by_table = a.r.rot ? kRotTable / (a.r.rot / 2) : kRotTokens;
   if (tt > by_table) tt = by_table;
+  if (tt > kRotTokens) tt = kRotTokens;
   if (tt < 1) tt = 1;
   a.tile_tokens = tt;
-  const long long grid = (a.tokens + tt - 1) / tt * a.head_tiles;
+  a.by_head = fast_div(per_head);
+  const long long grid = ((long long)a.tokens + tt - 1) / tt * a.head_tiles;
   if (grid > INT_MAX) return DSV4_ERR_UNSUPPORTED;
-  if (vec)
-    launch_k(rotary_kernel<T, V>, (unsigned)grid, kRotThreads, 0, st, a);
-  else
-    launch_k(rotary_kernel<T, 1>, (unsigned)grid, kRotThreads, 0, st, a);
+  auto kernel = vec ? (a.r.interleaved ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>)
+                    : (a.r.interleaved ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
+  launch_k(kernel, (unsigned)grid, kRotThreads, 0, st, a);
   return cudaGetLastError() == cudaSuccess ? DSV4_OK : DSV4_ERR_CUDA;
 }
 
@@ -273,7 +328,10 @@ int launch_rotary(const void* x, void* y, int dtype, const void* positions, int 
   a.pos64 = pos64;
   a.S = S;
   a.H = H;
-  a.tokens = (long long)B * S;
+  if ((long long)B * S > INT_MAX) return DSV4_ERR_UNSUPPORTED;
+  a.tokens = B * S;
+  // batches that follow each other like positions do are one run of positions
+  if (B == 1 || (xs[0] == S * xs[1] && ys[0] == S * ys[1])) a.S = a.tokens;
   a.in_place = x == y;
   a.inverse = inverse;
   a.amplitude = amplitude;
@@ -288,10 +346,9 @@ static int launch_cache_append_t(const AppendArgs& a, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   const bool vec = packs_ok(a.r, V) && a.row_stride % V == 0 && !(reinterpret_cast<uintptr_t>(a.rows) & 15);
   const unsigned grid = (unsigned)((a.T + kAppendRows - 1) / kAppendRows);
-  if (vec)
-    launch_k(cache_append_kernel<T, V>, grid, 32 * kAppendRows, 0, st, a);
-  else
-    launch_k(cache_append_kernel<T, 1>, grid, 32 * kAppendRows, 0, st, a);
+  auto kernel = vec ? (a.r.interleaved ? cache_append_kernel<T, V, true> : cache_append_kernel<T, V, false>)
+                    : (a.r.interleaved ? cache_append_kernel<T, 1, true> : cache_append_kernel<T, 1, false>);
+  launch_k(kernel, grid, 32 * kAppendRows, 0, st, a);
   return cudaGetLastError() == cudaSuccess ? DSV4_OK : DSV4_ERR_CUDA;
 }
 

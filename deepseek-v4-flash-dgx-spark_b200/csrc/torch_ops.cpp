@@ -19,6 +19,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <cerrno>
@@ -416,6 +417,43 @@ at::Tensor rotary(const at::Tensor& x, const at::Tensor& positions, const at::Te
   at::Tensor y = at::empty(v.sizes(), v.options());
   run_rotary(v, y, positions, freqs, interleaved, offset, inverse, amplitude);
   return y.view(x.sizes());
+}
+
+// The gradient of rotary is the rotation by the opposite angle.
+at::Tensor call_rotary(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
+                       std::optional<int64_t> offset, bool inverse, double amplitude) {
+  static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("dsv4moe::rotary", "").typed<decltype(rotary)>();
+  return op.call(x, positions, freqs, interleaved, offset, inverse, amplitude);
+}
+
+struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& positions,
+                            const at::Tensor& freqs, bool interleaved, std::optional<int64_t> offset, bool inverse,
+                            double amplitude) {
+    ctx->save_for_backward({positions, freqs});
+    ctx->saved_data["how"] = std::make_tuple(interleaved, offset.value_or(-1), inverse, amplitude);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_rotary(x, positions, freqs, interleaved, offset, inverse, amplitude);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto how = ctx->saved_data["how"].to<std::tuple<bool, int64_t, bool, double>>();
+    const std::optional<int64_t> offset =
+        std::get<1>(how) < 0 ? std::nullopt : std::optional<int64_t>(std::get<1>(how));
+    at::Tensor g;
+    if (grads[0].defined())
+      g = call_rotary(grads[0], saved[0], saved[1], std::get<0>(how), offset, !std::get<2>(how), std::get<3>(how));
+    return {g, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor rotary_autograd(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
+                           std::optional<int64_t> offset, bool inverse, double amplitude) {
+  if (at::GradMode::is_enabled() && x.requires_grad())
+    return RotaryFunction::apply(x, positions, freqs, interleaved, offset, inverse, amplitude);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_rotary(x, positions, freqs, interleaved, offset, inverse, amplitude);
 }
 
 void rotary_(at::Tensor x, const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
@@ -903,6 +941,10 @@ TORCH_LIBRARY_IMPL(dsv4moe, CUDA, m) {
   m.impl("cache_compact", &cache_compact);
   m.impl("cache_copy", &cache_copy);
   m.impl("paged_attn", &paged_attn);
+}
+
+TORCH_LIBRARY_IMPL(dsv4moe, Autograd, m) {
+  m.impl("rotary", &rotary_autograd);
 }
 
 // Ops without tensor inputs on a device (sizes, host reads) dispatch here.

@@ -41,7 +41,6 @@ def load():
             _lib.load()
             torch.ops.load_library(str(OPS_LIB))
             _register_fakes()
-            _register_gradients()
             _loaded = True
     return torch.ops.dsv4moe
 
@@ -139,19 +138,3 @@ def _register_fakes() -> None:
     for name in ("rotary_", "cache_append", "cache_reserve", "cache_free", "cache_fork", "cache_copy"):
         torch.library.register_fake(lib + name, lambda *args, **kwargs: None)
 
-
-def _register_gradients() -> None:
-    """The gradient of ``rotary`` is the rotation by the opposite angle."""
-
-    def setup_context(ctx, inputs, output):
-        _, positions, freqs, interleaved, offset, inverse, amplitude = inputs
-        ctx.save_for_backward(positions, freqs)
-        ctx.how = interleaved, offset, inverse, amplitude
-
-    def backward(ctx, grad):
-        positions, freqs = ctx.saved_tensors
-        interleaved, offset, inverse, amplitude = ctx.how
-        g = torch.ops.dsv4moe.rotary(grad, positions, freqs, interleaved, offset, not inverse, amplitude)
-        return g, None, None, None, None, None, None
-
-    torch.library.register_autograd("dsv4moe::rotary", backward, setup_context=setup_context)

@@ -306,7 +306,7 @@ DSV4_API int dsv4_sparse_attn(const void* q, const void* kv, const float* attn_s
  * x, y: [B,S,H,D] of dtype BF16, FP16 or FP32; strides of (b, s, h) in
  * elements, D contiguous; positions [B,S], int32 or (pos64) int64.  y == x with
  * equal strides rotates in place and touches the rotated channels only; any
- * other overlap is undefined.  rot <= 4096. */
+ * other overlap is undefined.  rot <= 4096, D <= 32760. */
 DSV4_API int dsv4_rotary(const void* x, void* y, int dtype, const void* positions, int pos64, const double* freqs,
                          int B, int S, int H, int D, int rot, int offset, int interleaved, int inverse,
                          float amplitude, const long long* x_strides, const long long* y_strides, void* stream);
