@@ -12,7 +12,7 @@
 // into a graph and need no copy of the tables on the host.
 //
 // The bookkeeping is a few hundred KB of integers and bound by latency: one CTA
-// of 1024 threads walks the page counts with ballots and one scan per 8192 pages,
+// of 1024 threads walks the page counts with ballots and one scan per 16384 pages (4096 in a small pool),
 // its results are the same in every run (free pages are taken in ascending order
 // and counts are integer sums), and the row copies follow as a second kernel over
 // all SMs, bound by HBM.
@@ -24,7 +24,7 @@ namespace dsv4 {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
-constexpr int kPlanStep = 8;  // pages per thread and scan step, their loads in flight together
+constexpr int kPlanShared = 4096;  // claims and offsets stay in shared memory up to so many sequences / entries
 
 // Exclusive scan of one int per thread over the CTA; *total gets the sum.
 // `scratch` is kPlanWarps + 1 ints of shared memory.
@@ -56,8 +56,10 @@ __device__ __forceinline__ int block_scan(int v, int* scratch, int* total) {
 }
 
 // Ascending ids p in [begin, end) with (refs[p] > 0) == used: their number, and
-// the ids themselves in list[0 .. limit).  Stops once `limit` are found.
-__device__ __forceinline__ int collect_pages(const int* refs, int begin, int end, bool used, int limit, int* list,
+// the ids themselves in list[0 .. limit).  Stops once `limit` are found.  kPlanStep
+// pages per thread and scan step have their loads in flight together.
+template <int kPlanStep>
+__device__ __forceinline__ int collect_step(const int* refs, int begin, int end, bool used, int limit, int* list,
                                              int* scratch) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int found = 0;
@@ -90,6 +92,12 @@ __device__ __forceinline__ int collect_pages(const int* refs, int begin, int end
   return found;
 }
 
+__device__ __forceinline__ int collect_pages(const int* refs, int begin, int end, bool used, int limit, int* list,
+                                             int* scratch) {
+  if (end - begin <= 4 * kPlanThreads) return collect_step<4>(refs, begin, end, used, limit, list, scratch);
+  return collect_step<16>(refs, begin, end, used, limit, list, scratch);
+}
+
 // Entry i's claim on sequence s: true for the first entry that names it.
 __device__ __forceinline__ void init_owners(int* owner, int n_seqs) {
   for (int s = threadIdx.x; s < n_seqs; s += blockDim.x) owner[s] = INT_MAX;
@@ -111,9 +119,10 @@ __device__ __forceinline__ int pages_of(int len, int page_size) {
 __global__ void __launch_bounds__(kPlanThreads) cache_reserve_kernel(const PageState st, const int* seqs,
                                                                      const int* new_lens, int n, int* ws) {
   __shared__ int scratch[kPlanWarps + 1];
-  int* owner = ws;
-  int* start = owner + st.n_seqs;
-  int* picked = start + n + 1;
+  __shared__ int owner_s[kPlanShared], start_s[kPlanShared + 1];
+  int* owner = st.n_seqs <= kPlanShared ? owner_s : ws;
+  int* start = n <= kPlanShared ? start_s : ws + st.n_seqs;
+  int* picked = ws + st.n_seqs + n + 1;
   init_owners(owner, st.n_seqs);
   for (int i = threadIdx.x; i < n; i += kPlanThreads) {
     const int s = seqs[i];
@@ -196,8 +205,9 @@ __global__ void __launch_bounds__(kPlanThreads) cache_fork_plan_kernel(const Pag
                                                                        const int* children, const int* fork_lens, int n,
                                                                        int* ws) {
   __shared__ int scratch[kPlanWarps + 1];
-  int* owner = ws;
-  int* len_of = owner + st.n_seqs;
+  __shared__ int owner_s[kPlanShared];
+  int* owner = st.n_seqs <= kPlanShared ? owner_s : ws;
+  int* len_of = ws + st.n_seqs;
   int* fresh = len_of + n;
   int* picked = fresh + n;
   init_owners(owner, st.n_seqs);

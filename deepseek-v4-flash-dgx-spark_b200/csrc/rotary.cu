@@ -168,8 +168,7 @@ constexpr int kRotThreads = 256;
 constexpr int kRotMax = 4096;     // rotated channels per head
 constexpr int kRotMaxDim = 32760;  // channels per head (FastDiv)
 constexpr int kRotTable = 2048;   // cosine / sine pairs a CTA keeps (16 KB)
-constexpr int kRotBatch = 4;      // units per thread, their loads in flight together
-constexpr int kRotUnits = kRotThreads * kRotBatch;
+constexpr int kRotPacks = 4;      // packs per thread, their loads in flight together
 constexpr int kRotTokens = 64;    // tokens a CTA takes at most
 
 // One CTA takes a tile of tokens x heads.  Every thread has its first units on the
@@ -187,6 +186,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
   const T* x = static_cast<const T*>(a.x);
   T* y = static_cast<T*>(a.y);
 
+  constexpr int kRotBatch = RotaryUnit<T, V, kInter>::kTwo ? kRotPacks / 2 : kRotPacks;
+  constexpr int kRotUnits = kRotThreads * kRotBatch;
   RotaryUnit<T, V, kInter> unit[kRotBatch];
   int at[kRotBatch], un[kRotBatch];  // token within the tile, unit of the head
   long long to[kRotBatch];           // where the head begins in y
@@ -294,7 +295,8 @@ static int launch_rotary_t(RotaryArgs a, cudaStream_t st) {
   const int n_rot = vec ? rotary_units<V>(a.r) : rotary_units<1>(a.r);
   const int per_head = a.in_place ? n_rot : vec ? head_units<V>(a.r) : head_units<1>(a.r);
   if (per_head == 0) return DSV4_OK;
-  // heads of a token first, then more tokens, up to kRotUnits units per CTA
+  // heads of a token first, then more tokens, up to a batch of units per thread
+  const int kRotUnits = kRotThreads * (vec && a.r.interleaved ? kRotPacks : kRotPacks / 2);
   a.tile_heads = kRotUnits / per_head < 1 ? 1 : kRotUnits / per_head;
   if (a.tile_heads > a.H) a.tile_heads = a.H;
   a.head_tiles = (a.H + a.tile_heads - 1) / a.tile_heads;
