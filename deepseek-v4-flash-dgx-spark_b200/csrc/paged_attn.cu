@@ -57,6 +57,8 @@ constexpr int kPaCtrl = 2048;
 constexpr int kPaSmemMax = 232448;                // shared memory a CTA may use
 constexpr int kPaMaxGrid = 1024;                  // CTAs (one per SM)
 constexpr int kPaTmemCols = 512;                  // S: two buffers of 64 columns; O^T at 256
+constexpr int kPaMinChunks = 2;                   // least chunks per CTA
+constexpr int kPaSnapChunks = 3;                  // a border moves so far to a row's begin or end
 constexpr float kPaRescaleLog2 = 10.0f;           // headroom of the running max, base 2
 constexpr float kPaNoMax = -3.402823466e38f;      // running max of a piece before its first key
 constexpr float kLog2e = 1.4426950408889634f;
@@ -69,11 +71,11 @@ struct PaArgs {
   const float* sink;      // [H] or NULL
   float* part_o;          // [grid][2][N][D]
   float* part_ml;         // [grid][2][N][2]: max (base 2), sum
-  int4* plan;             // [grid]: row, head group, boxes of the row before this CTA, boxes of the row
-  int* share;             // [1] boxes per CTA
+  int4* plan;             // [grid]: row, head group, boxes of the row before this CTA's border, boxes of the row
+  int* share;             // [1] boxes from border to border
   int T, H, D, groups;
   int n_seqs, max_pages, n_pages, page_log, box_log;
-  int idx64, window, first, stages, min_share;
+  int idx64, window, first, stages, min_share, snap;
   float scale;
 };
 
@@ -109,14 +111,28 @@ __device__ __forceinline__ int pa_box_key(const PaArgs& a, const PaRow& r, int b
   return (b < r.nfb ? b : b - r.nfb + r.wbb) << a.box_log;
 }
 
+// The list of `total` boxes is cut at every `share` boxes.  A border that falls less
+// than `snap` boxes from the begin or end of a row moves there: a piece of a row
+// costs its fp32 partials (256 KB written and read at 64 heads x 512), as much as
+// some chunks of keys.
+__device__ __forceinline__ int pa_share(int total, int ctas, int min_share) {
+  return max(total / ctas + (total % ctas != 0), min_share);
+}
+__device__ __forceinline__ int pa_snap(int o, int n, int snap) {
+  if (o <= 0) return 0;
+  if (o >= n) return n;
+  if (min(o, n - o) > snap) return o;
+  return o <= n - o ? 0 : n;
+}
+
 struct PaShared {
   uint64_t full[kPaMaxStages], empty[kPaMaxStages];
   uint64_t q_full[4], q_empty, s_full[2], s_free[2], p_ready[2], pv_done[2], last[2];
   uint32_t tmem;
   int abort;
   int t0, g0, i0;           // this CTA's first row, head group and box
-  long long left;           // boxes of its share
-  long long scan[kPaThreads / 32 + 1];
+  int begin, end;           // its boxes of the list
+  int scan[kPaThreads / 32];
   float red[2 * 64];        // one value per key half and head
   float m[64], f[64];       // max, factor per head
 };
@@ -260,83 +276,89 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  if (tid == 0) {
-    for (int i = 0; i < NST; ++i) {
-      mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 1);
+  // ---- this CTA's share of the box list -------------------------------------
+  const int per = (a.T + kPaThreads - 1) / kPaThreads;
+  const int r0 = min(a.T, tid * per), r1 = min(a.T, r0 + per);
+  int mine = 0;
+  for (int t = r0; t < r1; ++t) mine += pa_row(a, pa_index(a, t)).n * a.groups;
+  if (warp == 0) {
+    if (lane < NST) {
+      mbar_init(&sh.full[lane], 1);
+      mbar_init(&sh.empty[lane], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&sh.q_full[i], 1);
-    mbar_init(&sh.q_empty, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.s_free[i], kPaSoft / 32);
-      mbar_init(&sh.p_ready[i], kPaSoft / 32);
-      mbar_init(&sh.pv_done[i], 1);
+    if (lane < 4) mbar_init(&sh.q_full[lane], 1);
+    if (lane < 2) {
+      mbar_init(&sh.s_full[lane], 1);
+      mbar_init(&sh.s_free[lane], kPaSoft / 32);
+      mbar_init(&sh.p_ready[lane], kPaSoft / 32);
+      mbar_init(&sh.pv_done[lane], 1);
+      mbar_init(&sh.last[lane], 1);
     }
-    mbar_init(&sh.last[0], 1);
-    mbar_init(&sh.last[1], 1);
+    if (lane == 0) {
+      mbar_init(&sh.q_empty, 1);
+      sh.abort = 0;
+      sh.begin = sh.end = 0;
+      tma_prefetch_desc(&q_map);
+      tma_prefetch_desc(&kv_map);
+    }
     fence_barrier_init();
-    sh.abort = 0;
-    sh.left = 0;
   }
   if (warp == 1) {
     tmem_alloc(&sh.tmem, kPaTmemCols);
     tmem_relinquish();
   }
-
-  // ---- this CTA's share of the box list -------------------------------------
   {
-    const int per = (a.T + kPaThreads - 1) / kPaThreads;
-    const int r0 = min(a.T, tid * per), r1 = min(a.T, r0 + per);
-    long long mine = 0;
-    for (int t = r0; t < r1; ++t) mine += (long long)pa_row(a, pa_index(a, t)).n * a.groups;
-    long long inc = mine;
+    int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
     if (lane == 31) sh.scan[warp] = inc;
     __syncthreads();
-    if (tid == 0) {
-      long long run = 0;
-      for (int i = 0; i < kPaThreads / 32; ++i) {
-        const long long v = sh.scan[i];
-        sh.scan[i] = run;
-        run += v;
+    const int of_warp = lane < kPaThreads / 32 ? sh.scan[lane] : 0;
+    const int total = __reduce_add_sync(0xffffffffu, of_warp);
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0);
+    const int share = pa_share(total, (int)gridDim.x, a.min_share);
+    // borders blockIdx.x and blockIdx.x + 1 (past the list: its end)
+    const int at0 = before + inc - mine;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const long long far = (long long)share * ((int)blockIdx.x + x);
+      const int border = (int)min(far, (long long)total);
+      if (border == total && tid == 0) {
+        if (x) sh.end = total;
+        if (!x) sh.begin = total;
+        if (!x) a.plan[blockIdx.x] = make_int4(-1, 0, 0, 0);
       }
-      sh.scan[kPaThreads / 32] = run;
-    }
-    __syncthreads();
-    const long long total = sh.scan[kPaThreads / 32];
-    long long share = (total + gridDim.x - 1) / gridDim.x;
-    if (share < a.min_share) share = a.min_share;
-    const long long begin = share * blockIdx.x, end = min(total, begin + share);
-    long long at = sh.scan[warp] + inc - mine;
-    if (begin < end && at <= begin && begin < at + mine) {
+      if (border == total || border < at0 || border >= at0 + mine) continue;
+      int at = at0;
       for (int t = r0; t < r1; ++t) {
         const int n = pa_row(a, pa_index(a, t)).n;
-        if (begin < at + (long long)n * a.groups) {
-          sh.t0 = t;
-          sh.g0 = (int)((begin - at) / n);
-          sh.i0 = (int)((begin - at) % n);
-          sh.left = end - begin;
-          a.plan[blockIdx.x] = make_int4(t, sh.g0, sh.i0, n);
+        if (border < at + n * a.groups) {
+          const int g = (border - at) / n, o = border - at - g * n;
+          const int on = pa_snap(o, n, min(a.snap, share / 2));
+          if (x) {
+            sh.end = border - o + on;
+          } else {
+            sh.begin = border - o + on;
+            sh.t0 = t;
+            sh.g0 = g;
+            sh.i0 = on;
+            a.plan[blockIdx.x] = make_int4(t, g, o, n);
+          }
           break;
         }
-        at += (long long)n * a.groups;
+        at += n * a.groups;
       }
     }
-    if (tid == 0) {
-      if (begin >= end) a.plan[blockIdx.x] = make_int4(-1, 0, 0, 0);
-      if (blockIdx.x == 0) *a.share = (int)min(share, (long long)INT_MAX);
-    }
+    if (tid == 0 && blockIdx.x == 0) *a.share = share;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t t_s = __shfl_sync(0xffffffffu, sh.tmem, 0), t_o = t_s + 256;
-  long long left = __shfl_sync(0xffffffffu, sh.left, 0);
+  int left = __shfl_sync(0xffffffffu, sh.end - sh.begin, 0);
   int t = __shfl_sync(0xffffffffu, sh.t0, 0), g = __shfl_sync(0xffffffffu, sh.g0, 0);
   int i = __shfl_sync(0xffffffffu, sh.i0, 0);
   int2 sp = left > 0 ? pa_index(a, t) : make_int2(-1, -1);  // the row at hand; the next one's is loaded early
@@ -349,7 +371,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     while (left > 0 && ok && t < a.T) {
       const PaRow r = pa_row(a, sp);
       const int2 sp_next = pa_index(a, t + 1);
-      const int i1 = (int)min((long long)r.n, i + left);
+      const int i1 = min(r.n, i + left);
       if (i < i1) {
         const int* row = a.table + (long long)r.s * a.max_pages;
         left -= i1 - i;
@@ -442,7 +464,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     while (left > 0 && ok && t < a.T) {
       const int n = pa_row(a, sp).n;
       const int2 sp_next = pa_index(a, t + 1);
-      const int i1 = (int)min((long long)n, i + left);
+      const int i1 = min(n, i + left);
       if (i < i1) {
         left -= i1 - i;
         bool begin = true;
@@ -508,7 +530,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     while (left > 0 && ok && t < a.T) {
       const int n = pa_row(a, sp).n;
       const int2 sp_next = pa_index(a, t + 1);
-      const int i1 = (int)min((long long)n, i + left);
+      const int i1 = min(n, i + left);
       if (i < i1) {
         left -= i1 - i;
         bool begin = true;  // the piece's output starts anew
@@ -573,7 +595,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     while (left > 0 && t < a.T) {
       const PaRow r = pa_row(a, sp);
       const int2 sp_next = pa_index(a, t + 1);
-      const int i_begin = i, i1 = (int)min((long long)r.n, i + left);
+      const int i_begin = i, i1 = min(r.n, i + left);
       if (i < i1) {
         const int* pages = a.table + (long long)r.s * a.max_pages;
         left -= i1 - i;
@@ -766,31 +788,31 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   }
 }
 
-// Join the pieces of the rows that cross CTA borders.  Border c (CTA c begins inside
-// a row) is a row's first if the row begins in CTA c - 1; the row's pieces are then
-// CTA c - 1's second kind (the one that holds its begin) and the first kind of CTAs
-// c, c + 1, ...  Every CTA lists those rows from the plan, and the work units (row,
-// head, 128 channels) go round the warps of the grid: one warp per unit, or all
-// eight of a CTA, each on every eighth piece, where the units are few (one long row
-// left in 65 pieces: 64 heads x 4 units).
+// Join the pieces of the rows that cross CTA borders.  Border c is a row's first if it
+// lies inside the row and the border before does not; the row's pieces are then CTA
+// c - 1's second kind (the one that holds its begin) and the first kind of CTAs c,
+// c + 1, ...  Every CTA lists those rows from the plan, and the work units (row, head)
+// go round the warps of the grid: one warp per unit, or all eight of a CTA, each on
+// every eighth piece, where the units are few.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
-constexpr int kJoinAhead = 8;  // pieces whose loads are in flight together
+constexpr int kJoinAhead = 4;  // pieces whose loads are in flight together
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaArgs a, int n_plan) {
-  __shared__ int4 rows[kPaMaxGrid];   // row, head group, first piece, pieces
+  __shared__ int4 rows[kPaMaxGrid];   // row, head group, first piece's CTA, pieces
   __shared__ int count[kJoinWarps];
-  __shared__ float red[kJoinWarps][32][4];
+  __shared__ float4 red[kJoinWarps][4][32];
   __shared__ float den_of[kJoinWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long share = *a.share;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, DT = a.D / 128;
+  const int share = *a.share, snap = min(a.snap, share / 2);
   int n_rows = 0;  // in border order, so that every CTA has the same list
   for (int base = 1; base < n_plan; base += kJoinThreads) {
     const int c = base + threadIdx.x;
-    int4 pl = make_int4(-1, 0, 0, 0);  // row, group, boxes before the border, boxes of the row
+    int4 pl = make_int4(-1, 0, 0, 0);
     if (c < n_plan) pl = a.plan[c];
-    const bool on = pl.x >= 0 && pl.z > 0 && pl.z <= share;
+    auto inside = [&](int o) { return o > 0 && o < pl.w && pa_snap(o, pl.w, snap) == o; };
+    const bool on = pl.x >= 0 && inside(pl.z) && !inside(pl.z - share);
     const unsigned vote = __ballot_sync(0xffffffffu, on);
     if (lane == 0) count[warp] = __popc(vote);
     __syncthreads();
@@ -799,73 +821,95 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaA
       if (w < warp) at += count[w];
       n_rows += count[w];
     }
-    if (on) rows[at + __popc(vote & ((1u << lane) - 1))] = make_int4(pl.x, pl.y, c - 1, 2 + (int)((pl.w - pl.z - 1) / share));
+    if (on) {
+      int more = (pl.w - pl.z - 1) / share;  // borders of the row behind this one
+      if (more && !inside(pl.z + more * share)) --more;
+      rows[at + __popc(vote & ((1u << lane) - 1))] = make_int4(pl.x, pl.y, c - 1, 2 + more);
+    }
     __syncthreads();
   }
-  const int slices = a.D / 128;
-  const long long units = (long long)n_rows * N * slices;
-  const bool together = units * kJoinWarps <= (long long)gridDim.x * kJoinWarps;
-  const long long first = together ? blockIdx.x : (long long)blockIdx.x * kJoinWarps + warp;
-  const long long step = together ? gridDim.x : (long long)gridDim.x * kJoinWarps;
-  for (long long u = first; u < units; u += step) {
-    const int slice = (int)(u % slices), h = (int)(u / slices % N);
-    const int4 r = rows[u / slices / N];
+  const int units = n_rows * N;
+  const bool together = units <= (int)gridDim.x;
+  const int first = together ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
+  const int step = together ? gridDim.x : gridDim.x * kJoinWarps;
+  for (int u = first; u < units; u += step) {
+    const int h = u % N;
+    const int4 r = rows[u / N];
     const int head = 64 * r.y + h;
     if (head >= a.H) continue;
-    auto piece = [&](int i) { return (size_t)r.z * 2 + (i == 0 ? 1 : 2 * i); };
-    // each lane holds the maxima and sums of pieces lane, lane + 32, ...
+    auto piece = [&](int i) { return ((size_t)r.z * 2 + (i == 0 ? 1 : 2 * i)) * N + h; };
+    // each lane holds the maxima of pieces lane, lane + 32, ...
     const float sk = a.sink ? __ldg(a.sink + head) * kLog2e : -INFINITY;
-    float mx = sk;
-    for (int i = lane; i < r.w; i += 32) mx = fmaxf(mx, a.part_ml[(piece(i) * N + h) * 2]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    float den = 0.f, acc[4] = {};
     const int p0 = together ? warp : 0, ps = together ? kJoinWarps : 1;
-    for (int i0 = p0; i0 < r.w; i0 += ps * kJoinAhead) {
-      float4 o[kJoinAhead];
-      float f[kJoinAhead];
+    float4 o[kJoinAhead][4];
+    float2 ml[kJoinAhead];
+    auto load = [&](int i0) {
 #pragma unroll
       for (int j = 0; j < kJoinAhead; ++j) {
         const int i = i0 + j * ps;
-        f[j] = 0.f;
         if (i >= r.w) continue;
-        const size_t at = piece(i) * N + h;
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-        o[j] = *reinterpret_cast<const float4*>(a.part_o + at * a.D + 128 * slice + 4 * lane);
-        if (ml.x != kPaNoMax) {
-          f[j] = ex2(ml.x - mx);
-          den += ml.y * f[j];
-        }
+        const size_t at = piece(i);
+        ml[j] = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (x < DT) o[j][x] = *reinterpret_cast<const float4*>(a.part_o + at * a.D + 128 * x + 4 * lane);
       }
+    };
+    load(p0);  // on the way while the maxima are compared
+    float mx = sk;
+    for (int i = lane; i < r.w; i += 32) mx = fmaxf(mx, a.part_ml[piece(i) * 2]);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+    float den = 0.f;
+    float4 acc[4] = {};
+    for (int i0 = p0; i0 < r.w; i0 += ps * kJoinAhead) {
+      if (i0 != p0) load(i0);
 #pragma unroll
       for (int j = 0; j < kJoinAhead; ++j) {
-        if (f[j] == 0.f) continue;
-        acc[0] += o[j].x * f[j];
-        acc[1] += o[j].y * f[j];
-        acc[2] += o[j].z * f[j];
-        acc[3] += o[j].w * f[j];
+        if (i0 + j * ps >= r.w || ml[j].x == kPaNoMax) continue;
+        const float f = ex2(ml[j].x - mx);
+        den += ml[j].y * f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (x >= DT) break;
+          acc[x].x += o[j][x].x * f;
+          acc[x].y += o[j][x].y * f;
+          acc[x].z += o[j][x].z * f;
+          acc[x].w += o[j][x].w * f;
+        }
       }
     }
     if (together) {
       __syncthreads();
 #pragma unroll
-      for (int x = 0; x < 4; ++x) red[warp][lane][x] = acc[x];
+      for (int x = 0; x < 4; ++x)
+        if (x < DT) red[warp][x][lane] = acc[x];
       if (lane == 0) den_of[warp] = den;
       __syncthreads();
-      if (warp) continue;
-      for (int w = 1; w < kJoinWarps; ++w) {
+      if (warp >= DT) continue;
+      // warp x adds up channels 128 x .. +127
+      den = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < kJoinWarps; ++w) {
         den += den_of[w];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) acc[x] += red[w][lane][x];
+        const float4 v = red[w][warp][lane];
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
       }
+      acc[0] = sum;
     }
-    const bool any = den > 0.f || den != den;
+    const bool any = den != 0.f;
     den += ex2(sk - mx);
-    Pack<T, 4> out;
+    const float inv = any ? 1.f / den : 0.f;
+    T* dst = static_cast<T*>(a.out) + ((size_t)r.x * a.H + head) * a.D + (together ? 128 * warp : 0) + 4 * lane;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) out.v[x] = from_f32<T>(any ? acc[x] / den : 0.f);
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + ((size_t)r.x * a.H + head) * a.D + 128 * slice + 4 * lane) =
-        *reinterpret_cast<const uint2*>(&out);
+    for (int x = 0; x < 4; ++x) {
+      if (x >= (together ? 1 : DT)) break;
+      *reinterpret_cast<uint2*>(dst + 128 * x) =
+          make_uint2(pack2<T>(acc[x].x * inv, acc[x].y * inv), pack2<T>(acc[x].z * inv, acc[x].w * inv));
+    }
   }
 }
 
@@ -888,10 +932,10 @@ static PaShape pa_shape(int T, int H, int D, long long max_keys, int num_sms) {
   const long long most = (long long)T * s.groups * ((max_keys + kPaChunk - 1) / kPaChunk);
   if (num_sms > kPaMaxGrid) num_sms = kPaMaxGrid;
   s.grid = (int)(most < num_sms ? (most < 1 ? 1 : most) : num_sms);
-  // a unit per warp for every row that may be split, up to eight CTAs per SM
+  // a CTA for every head of a row that may be split, up to four per SM
   const long long split = s.grid - 1 < (long long)T * s.groups ? s.grid - 1 : (long long)T * s.groups;
-  const long long units = split * s.N * (D / 128);
-  s.join_grid = (int)(units < 8LL * num_sms ? (units < 1 ? 1 : units) : 8LL * num_sms);
+  const long long units = split * s.N;
+  s.join_grid = (int)(units < 4LL * num_sms ? (units < 1 ? 1 : units) : 4LL * num_sms);
   return s;
 }
 
@@ -935,6 +979,9 @@ int launch_paged_attn(const void* q, bool fp16, int T, int H, int D, long long q
   const long long max_keys = (long long)max_pages * page_size;
   if (paged_attn_workspace(T, H, D, max_keys, num_sms) > ws_bytes || !ws) return DSV4_ERR_WORKSPACE;
   const PaShape s = pa_shape(T, H, D, max_keys, num_sms);
+  // the kernel counts boxes (page_size rows, at most 64) of all rows in 32 bits
+  const int box = page_size < kPaChunk ? page_size : kPaChunk;
+  if ((long long)T * s.groups * (max_keys / box + 1) > INT_MAX) return DSV4_ERR_UNSUPPORTED;
   CUtensorMap qm, kvm;
   int rc = make_tmap_rows16(&qm, fp16, q, D, H, q_stride_h, T, q_stride_t, s.N);
   if (rc == DSV4_OK)
@@ -964,7 +1011,8 @@ int launch_paged_attn(const void* q, bool fp16, int T, int H, int D, long long q
   a.window = window;
   a.first = first;
   a.stages = s.stages;
-  a.min_share = kPaChunk >> a.box_log;  // a chunk
+  a.min_share = kPaMinChunks * (kPaChunk >> a.box_log);
+  a.snap = kPaSnapChunks * (kPaChunk >> a.box_log);
   a.scale = scale;
   if (fp16) {
     if (s.N == 64) return launch_paged_attn_t<__half, 64>(s, qm, kvm, a, st);

@@ -379,7 +379,9 @@ DSV4_API int dsv4_cache_copy(void* pages, int n_layers, int D, long long layer_s
  * with no key, gives zeros.  What hidden rows of a page hold (NaN included) has
  * no effect.  out [T,H,D].
  * H <= 128; D = 128, 256 or 512; page_size a power of two from 16 on; BF16 or
- * FP16; all 16-byte aligned (DSV4_ERR_UNSUPPORTED / DSV4_ERR_ARG otherwise).
+ * FP16; all 16-byte aligned; T x (H / 64, rounded up) x max_pages x
+ * page_size / min(page_size, 64) below 2^31 (DSV4_ERR_UNSUPPORTED / DSV4_ERR_ARG
+ * otherwise).
  * Two calls may share a workspace only if they do not overlap on the GPU. */
 DSV4_API long long dsv4_paged_attn_workspace_bytes(int T, int H, int D, int page_size, int max_pages);
 DSV4_API int dsv4_paged_attn(const void* q, long long q_stride_t, long long q_stride_h, int dtype, int T, int H,
