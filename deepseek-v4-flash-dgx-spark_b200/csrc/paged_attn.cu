@@ -57,7 +57,7 @@ constexpr int kPaCtrl = 2048;
 constexpr int kPaSmemMax = 232448;                // shared memory a CTA may use
 constexpr int kPaMaxGrid = 1024;                  // CTAs (one per SM)
 constexpr int kPaTmemCols = 512;                  // S: two buffers of 64 columns; O^T at 256
-constexpr int kPaMinChunks = 2;                   // least chunks per CTA
+constexpr int kPaMinChunks = 1;                   // least chunks per CTA
 constexpr int kPaSnapChunks = 3;                  // a border moves so far to a row's begin or end
 constexpr float kPaRescaleLog2 = 10.0f;           // headroom of the running max, base 2
 constexpr float kPaNoMax = -3.402823466e38f;      // running max of a piece before its first key
@@ -240,11 +240,13 @@ __host__ __device__ constexpr uint32_t pa_idesc(uint32_t m, uint32_t n, uint32_t
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-__device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z) {
+// Rows of both maps are split into 64-channel tiles: coordinates (0, row, tile, page or token).
+__device__ __forceinline__ void tma_load_tiles(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int row, int tile,
+                                               int z) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(tile), "r"(z)
       : "memory");
 }
 
@@ -255,6 +257,23 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   memcpy(&x, &a, 2);
   memcpy(&y, &b, 2);
   return (uint32_t)x | ((uint32_t)y << 16);
+}
+
+// Lane l of four holds column l of four rows; it gets row l % 4 of the four columns.
+__device__ __forceinline__ float4 transpose4(float a0, float a1, float a2, float a3, int lane) {
+  const bool o1 = lane & 1, o2 = lane & 2;
+  const float r0 = __shfl_xor_sync(0xffffffffu, o1 ? a0 : a1, 1);
+  const float r1 = __shfl_xor_sync(0xffffffffu, o1 ? a2 : a3, 1);
+  if (o1) {
+    a0 = r0;
+    a2 = r1;
+  } else {
+    a1 = r0;
+    a3 = r1;
+  }
+  const float s0 = __shfl_xor_sync(0xffffffffu, o2 ? a0 : a2, 2);
+  const float s1 = __shfl_xor_sync(0xffffffffu, o2 ? a1 : a3, 2);
+  return o2 ? make_float4(s0, s1, a2, a3) : make_float4(a0, a1, s0, s1);
 }
 
 // N: heads per group, padded to 16, 32 or 64 (rows past H load as zeros).  The score
@@ -279,8 +298,12 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   // ---- this CTA's share of the box list -------------------------------------
   const int per = (a.T + kPaThreads - 1) / kPaThreads;
   const int r0 = min(a.T, tid * per), r1 = min(a.T, r0 + per);
-  int mine = 0;
-  for (int t = r0; t < r1; ++t) mine += pa_row(a, pa_index(a, t)).n * a.groups;
+  int mine = 0, n_r0 = 0;  // boxes of this thread's rows, and of the first
+  for (int t = r0; t < r1; ++t) {
+    const int n = pa_row(a, pa_index(a, t)).n;
+    if (t == r0) n_r0 = n;
+    mine += n * a.groups;
+  }
   if (warp == 0) {
     if (lane < NST) {
       mbar_init(&sh.full[lane], 1);
@@ -322,34 +345,35 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     const int share = pa_share(total, (int)gridDim.x, a.min_share);
     // borders blockIdx.x and blockIdx.x + 1 (past the list: its end)
     const int at0 = before + inc - mine;
-#pragma unroll
+#pragma unroll 1
     for (int x = 0; x < 2; ++x) {
-      const long long far = (long long)share * ((int)blockIdx.x + x);
-      const int border = (int)min(far, (long long)total);
+      const int border = (int)min((long long)share * ((int)blockIdx.x + x), (long long)total);
       if (border == total && tid == 0) {
         if (x) sh.end = total;
         if (!x) sh.begin = total;
         if (!x) a.plan[blockIdx.x] = make_int4(-1, 0, 0, 0);
       }
       if (border == total || border < at0 || border >= at0 + mine) continue;
-      int at = at0;
-      for (int t = r0; t < r1; ++t) {
-        const int n = pa_row(a, pa_index(a, t)).n;
-        if (border < at + n * a.groups) {
-          const int g = (border - at) / n, o = border - at - g * n;
-          const int on = pa_snap(o, n, min(a.snap, share / 2));
-          if (x) {
-            sh.end = border - o + on;
-          } else {
-            sh.begin = border - o + on;
-            sh.t0 = t;
-            sh.g0 = g;
-            sh.i0 = on;
-            a.plan[blockIdx.x] = make_int4(t, g, o, n);
-          }
-          break;
-        }
+      int at = at0, t = r0, n = n_r0;  // the row that holds it
+      while (border >= at + n * a.groups) {
         at += n * a.groups;
+        ++t;
+        n = pa_row(a, pa_index(a, t)).n;
+      }
+      int g = 0, o = border - at;
+      while (o >= n) {
+        o -= n;
+        ++g;
+      }
+      const int on = pa_snap(o, n, min(a.snap, share >> 1));
+      if (x) {
+        sh.end = border - o + on;
+      } else {
+        sh.begin = border - o + on;
+        sh.t0 = t;
+        sh.g0 = g;
+        sh.i0 = on;
+        a.plan[blockIdx.x] = make_int4(t, g, o, n);
       }
     }
     if (tid == 0 && blockIdx.x == 0) *a.share = share;
@@ -388,9 +412,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           q_issued = true;
           if (lane < DT) {
             mbar_arrive_expect_tx(&sh.q_full[lane], 2 * N * 128);
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-              tma_load_3d_at(smem_u32(sQ + (2 * lane + x) * N * 128), &q_map, &sh.q_full[lane], 128 * lane + 64 * x, 64 * g, t);
+            tma_load_tiles(smem_u32(sQ + 2 * lane * N * 128), &q_map, &sh.q_full[lane], 64 * g, 2 * lane, t);
           }
           __syncwarp();
         };
@@ -416,8 +438,8 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             if (on) {
               const uint32_t dst = smem_u32(ring + slot * kPaStage) + (lane << (a.box_log + 7));
               const int y = key & ((1 << a.page_log) - 1);
-              tma_load_3d_at(dst, &kv_map, &sh.full[slot], 128 * dt, y, page_now);
-              tma_load_3d_at(dst + kPaTile, &kv_map, &sh.full[slot], 128 * dt + 64, y, page_now);
+              tma_load_tiles(dst, &kv_map, &sh.full[slot], y, 2 * dt, page_now);
+              if (nsub > 1) tma_load_tiles(dst + kPaTile, &kv_map, &sh.full[slot], y, 2 * dt + 1, page_now);
             }
             ++issued;
             if (++slot == NST) {
@@ -438,6 +460,9 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         sp = sp_next;
       }
     }
+    // the join may be launched once every CTA is here: its start then overlaps the last
+    // chunks (any earlier, its CTAs crowd the SMs that this grid leaves free)
+    if (lane == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // every copy has landed before the CTA can exit, also when a wait ran out
     for (int k = 0; k < min(issued, NST); ++k) {
       if (slot == 0) {
@@ -759,10 +784,17 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           tmem_ldn<HPT>(t_o + N * dt + h0 + lane_base, o);
           const int d = 128 * dt + row;
           if (whole) {
-            T* dst = out + ((size_t)t * a.H + 64 * g + h0) * a.D + d;
+            // four lanes exchange four heads each, so that a thread has four channels of
+            // one head: 8-byte stores instead of 2-byte ones, which take 4 cycles each
 #pragma unroll
-            for (int x = 0; x < HPT; ++x)
-              if (h0 + x < heads) dst[(size_t)x * a.D] = from_f32<T>(o[x] * sh.f[h0 + x]);
+            for (int x = 0; x < HPT; x += 4) {
+              const float4 v = transpose4(o[x], o[x + 1], o[x + 2], o[x + 3], lane);
+              const int h = h0 + x + (lane & 3);
+              const float f = sh.f[h];
+              if (h < heads)
+                *reinterpret_cast<uint2*>(out + ((size_t)t * a.H + 64 * g + h) * a.D + (d & ~3)) =
+                    make_uint2(pack2<T>(v.x * f, v.y * f), pack2<T>(v.z * f, v.w * f));
+            }
           } else {
             float* dst = a.part_o + (piece * N + h0) * a.D + d;
 #pragma unroll
@@ -796,6 +828,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 // every eighth piece, where the units are few.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinSpread = 120 * 1024;  // shared memory that keeps a second CTA off the SM
 constexpr int kJoinAhead = 4;  // pieces whose loads are in flight together
 
 template <typename T, int N>
@@ -805,6 +838,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaA
   __shared__ float4 red[kJoinWarps][4][32];
   __shared__ float den_of[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, DT = a.D / 128;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // all of the attention's stores
   const int share = *a.share, snap = min(a.snap, share / 2);
   int n_rows = 0;  // in border order, so that every CTA has the same list
   for (int base = 1; base < n_plan; base += kJoinThreads) {
@@ -946,16 +980,17 @@ long long paged_attn_workspace(int T, int H, int D, long long max_keys, int num_
   return pa_pieces_bytes(s, D) + (long long)s.grid * 16 + 16;
 }
 
-// 16-bit elements [z][y][64-channel tiles], 128-byte swizzled boxes of rows x 64 channels.
-static int make_tmap_rows16(CUtensorMap* m, bool fp16, const void* base, int channels, int y, long long y_stride, int z,
-                            long long z_stride, int box_rows) {
+// 16-bit rows as {64 channels, rows, 64-channel tiles, z}: a box of `tiles` tiles x
+// box_rows rows lands as [tile][row][64 channels], 128-byte swizzled.
+static int make_tmap_tiles16(CUtensorMap* m, bool fp16, const void* base, int channels, int rows, long long row_stride,
+                             int z, long long z_stride, int box_rows, int tiles) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return DSV4_ERR_CUDA;
-  cuuint64_t dims[3] = {(cuuint64_t)channels, (cuuint64_t)y, (cuuint64_t)z};
-  cuuint64_t strides[2] = {(cuuint64_t)y_stride * 2, (cuuint64_t)z_stride * 2};
-  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
-  cuuint32_t es[3] = {1, 1, 1};
-  const CUresult r = enc(m, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+  cuuint64_t dims[4] = {64, (cuuint64_t)rows, (cuuint64_t)(channels / 64), (cuuint64_t)z};
+  cuuint64_t strides[3] = {(cuuint64_t)row_stride * 2, 128, (cuuint64_t)z_stride * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)tiles, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r = enc(m, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                          const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -964,10 +999,31 @@ static int make_tmap_rows16(CUtensorMap* m, bool fp16, const void* base, int cha
 
 template <typename T, int N>
 static int launch_paged_attn_t(const PaShape& s, const CUtensorMap& qm, const CUtensorMap& kvm, const PaArgs& a,
-                               cudaStream_t st) {
+                               int num_sms, cudaStream_t st) {
   if (ensure_smem_attr(reinterpret_cast<const void*>(paged_attn_kernel<T, N>), (int)s.smem)) return DSV4_ERR_CUDA;
   launch_k(paged_attn_kernel<T, N>, s.grid, kPaThreads, s.smem, st, qm, kvm, a);
-  if (s.grid > 1) launch_k(paged_attn_join_kernel<T, N>, s.join_grid, kJoinThreads, 0, st, a, s.grid);
+  if (s.grid > 1) {
+    // launched while the attention ends: its CTAs take the SMs' places as they get free
+    // and wait there for the whole grid (griddepcontrol.wait); few CTAs get an SM each
+    const size_t spread = s.join_grid <= num_sms ? kJoinSpread : 0;
+    if (spread && ensure_smem_attr(reinterpret_cast<const void*>(paged_attn_join_kernel<T, N>), (int)spread))
+      return DSV4_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)s.join_grid);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = st;
+    cfg.dynamicSmemBytes = spread;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    count_launch();
+    if (cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T, N>, a, s.grid) != cudaSuccess) {
+      cudaGetLastError();
+      return DSV4_ERR_CUDA;
+    }
+  }
   return cudaGetLastError() == cudaSuccess ? DSV4_OK : DSV4_ERR_CUDA;
 }
 
@@ -983,10 +1039,9 @@ int launch_paged_attn(const void* q, bool fp16, int T, int H, int D, long long q
   const int box = page_size < kPaChunk ? page_size : kPaChunk;
   if ((long long)T * s.groups * (max_keys / box + 1) > INT_MAX) return DSV4_ERR_UNSUPPORTED;
   CUtensorMap qm, kvm;
-  int rc = make_tmap_rows16(&qm, fp16, q, D, H, q_stride_h, T, q_stride_t, s.N);
+  int rc = make_tmap_tiles16(&qm, fp16, q, D, H, q_stride_h, T, q_stride_t, s.N, 2);
   if (rc == DSV4_OK)
-    rc = make_tmap_rows16(&kvm, fp16, pages, D, page_size, D, n_pages, page_stride,
-                          page_size < kPaChunk ? page_size : kPaChunk);
+    rc = make_tmap_tiles16(&kvm, fp16, pages, D, page_size, D, n_pages, page_stride, box, box == kPaChunk ? 2 : 1);
   if (rc != DSV4_OK) return rc;
   PaArgs a{};
   a.out = out;
@@ -1015,13 +1070,13 @@ int launch_paged_attn(const void* q, bool fp16, int T, int H, int D, long long q
   a.snap = kPaSnapChunks * (kPaChunk >> a.box_log);
   a.scale = scale;
   if (fp16) {
-    if (s.N == 64) return launch_paged_attn_t<__half, 64>(s, qm, kvm, a, st);
-    if (s.N == 32) return launch_paged_attn_t<__half, 32>(s, qm, kvm, a, st);
-    return launch_paged_attn_t<__half, 16>(s, qm, kvm, a, st);
+    if (s.N == 64) return launch_paged_attn_t<__half, 64>(s, qm, kvm, a, num_sms, st);
+    if (s.N == 32) return launch_paged_attn_t<__half, 32>(s, qm, kvm, a, num_sms, st);
+    return launch_paged_attn_t<__half, 16>(s, qm, kvm, a, num_sms, st);
   }
-  if (s.N == 64) return launch_paged_attn_t<__nv_bfloat16, 64>(s, qm, kvm, a, st);
-  if (s.N == 32) return launch_paged_attn_t<__nv_bfloat16, 32>(s, qm, kvm, a, st);
-  return launch_paged_attn_t<__nv_bfloat16, 16>(s, qm, kvm, a, st);
+  if (s.N == 64) return launch_paged_attn_t<__nv_bfloat16, 64>(s, qm, kvm, a, num_sms, st);
+  if (s.N == 32) return launch_paged_attn_t<__nv_bfloat16, 32>(s, qm, kvm, a, num_sms, st);
+  return launch_paged_attn_t<__nv_bfloat16, 16>(s, qm, kvm, a, num_sms, st);
 }
 
 }  // namespace dsv4
