@@ -24,7 +24,7 @@ namespace dsv4 {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
-constexpr int kPlanShared = 4096;  // claims and offsets stay in shared memory up to so many sequences / entries
+constexpr int kPlanShared = 2048;  // claims and offsets stay in shared memory up to so many sequences / entries
 
 // Exclusive scan of one int per thread over the CTA; *total gets the sum.
 // `scratch` is kPlanWarps + 1 ints of shared memory.
@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_reserve_kernel(const PageS
                                                                      const int* new_lens, int n, int* ws) {
   __shared__ int scratch[kPlanWarps + 1];
   __shared__ int owner_s[kPlanShared], start_s[kPlanShared + 1];
+  __shared__ long long row_s[kPlanShared];  // where page k of the call goes in the table, less k
   int* owner = st.n_seqs <= kPlanShared ? owner_s : ws;
   int* start = n <= kPlanShared ? start_s : ws + st.n_seqs;
   int* picked = ws + st.n_seqs + n + 1;
@@ -147,6 +148,8 @@ __global__ void __launch_bounds__(kPlanThreads) cache_reserve_kernel(const PageS
     const int at = block_scan(need, scratch, &sum);
     // past n_pages the exact sum no longer matters: the call is refused
     if (i < n) start[i] = (int)min(total + at, (long long)INT_MAX);
+    if (i < n && need && i < kPlanShared)
+      row_s[i] = (long long)seqs[i] * st.max_pages + pages_of(st.lens[seqs[i]], st.page_size) - start[i];
     total = min(total + sum, (long long)INT_MAX);
   }
   if (threadIdx.x == 0) start[n] = (int)total;
@@ -155,18 +158,25 @@ __global__ void __launch_bounds__(kPlanThreads) cache_reserve_kernel(const PageS
     if (threadIdx.x == 0) record_error(DSV4_DEVERR_NO_PAGES);
     return;
   }
-  // a warp per entry, or several where the entries are few
+  // a warp per entry, or several where the entries are few; four pages per lane in flight
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int share = n < kPlanWarps ? kPlanWarps / n : 1;
-  for (int e = w; e < n * share; e += kPlanWarps) {
-    const int i = e / share, from = start[i], to = start[i + 1];
+  const int warps = n < kPlanWarps ? kPlanWarps / n : 1;
+  for (int e = w; e < n * warps; e += kPlanWarps) {
+    const int i = e / warps, from = start[i], to = start[i + 1];
     if (from == to) continue;
-    const int s = seqs[i];
-    int* row = st.table + (long long)s * st.max_pages + pages_of(st.lens[s], st.page_size) - from;
-    for (int k = from + (e % share) * 32 + lane; k < to; k += 32 * share) {
-      const int p = picked[k];
-      row[k] = p;
-      st.refs[p] = 1;
+    const long long at = i < kPlanShared
+                             ? row_s[i]
+                             : (long long)seqs[i] * st.max_pages + pages_of(st.lens[seqs[i]], st.page_size) - from;
+    for (int k0 = from + (e % warps) * 128 + lane; k0 < to; k0 += 128 * warps) {
+      int p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = k0 + 32 * j < to ? picked[k0 + 32 * j] : -1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (p[j] < 0) continue;
+        st.table[at + k0 + 32 * j] = p[j];
+        st.refs[p[j]] = 1;
+      }
     }
   }
   __syncthreads();

@@ -33,6 +33,8 @@ _loaded = False
 def load():
     """Load the op library once and return the ``torch.ops.dsv4moe`` namespace."""
     global _loaded
+    if _loaded:
+        return torch.ops.dsv4moe
     with _lock:
         if not _loaded:
             if not OPS_LIB.exists():
