@@ -178,6 +178,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The sink's weight against the max (1 where it is the max, also an infinite one).
+__device__ __forceinline__ float pa_sink(float sink, float mx) { return sink == mx ? 1.f : ex2(sink - mx); }
+
 // n consecutive fp32 columns of this thread's TMEM lane, n = 8, 16 or 32.
 template <int n>
 __device__ __forceinline__ void tmem_ldn(uint32_t taddr, float (&v)[n]) {
@@ -771,7 +774,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           if (whole) {
             const float sk = a.sink && st < heads ? __ldg(a.sink + 64 * g + st) * kLog2e : -INFINITY;
             const float mx = fmaxf(m, sk);
-            const float den = l * ex2(m - mx) + ex2(sk - mx);
+            const float den = l * ex2(m - mx) + pa_sink(sk, mx);
             sh.f[st] = m == kPaNoMax ? 0.f : ex2(m - mx) / den;
           } else {
             a.part_ml[(piece * N + st) * 2] = m;
@@ -935,7 +938,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaA
       acc[0] = sum;
     }
     const bool any = den != 0.f;
-    den += ex2(sk - mx);
+    den += pa_sink(sk, mx);
     const float inv = any ? 1.f / den : 0.f;
     T* dst = static_cast<T*>(a.out) + ((size_t)r.x * a.H + head) * a.D + (together ? 128 * warp : 0) + 4 * lane;
 #pragma unroll

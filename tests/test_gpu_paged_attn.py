@@ -183,6 +183,22 @@ def test_visible_infinities_and_nan_stay_in_their_row(cuda_device):
     _check(out[::2], q[::2], lambda t, keys: c.rows[2 * t][keys], [199, 199], None, 0.05, 0, 0)
 
 
+def test_extreme_sinks(cuda_device):
+    """A sink of +inf takes all the weight, one of -inf none, in whole rows and in rows
+    joined from pieces."""
+    from spark_b200 import kv_cache
+
+    c = Cache([40, 3000], 64, 512, torch.bfloat16, seed=7)
+    q = torch.randn(2, 64, 512, generator=c.g, device="cuda").bfloat16()
+    sink = torch.randn(64, generator=c.g, device="cuda")
+    sink[3], sink[5], sink[6], sink[7] = float("inf"), float("-inf"), 200.0, -200.0
+    pos = torch.tensor([39, 2999], device="cuda")
+    out = kv_cache.paged_attn(q, c.pages, c.table, None, pos, sink, 0.05)
+    assert torch.all(out[:, 3] == 0)
+    keep = [h for h in range(64) if h != 3]
+    _check(out[:, keep], q[:, keep], lambda t, keys: c.rows[t][keys], [39, 2999], sink[keep], 0.05, 0, 0)
+
+
 def test_strides_and_layouts(cuda_device):
     from spark_b200 import kv_cache
 
