@@ -20,10 +20,14 @@
 // Bound: a row of D = 512 is 1 KB from HBM and 131 kFLOP with 64 heads.  Issued
 // from warp-uniform code the two products cost 36 and 51 cycles per instruction
 // (measured), 1970 cycles per chunk, against 2840 at which an SM's share of HBM
-// delivers the chunk's 64 KB: the cache can stream at the HBM rate as long as the
-// loads never pause.  Chunks of 128 keys cost fewer tensor cycles per key but hold
-// all of the ring until their softmax is done: the loads then stand still for half
-// of the time (measured: 353 against 291 us for 16 rows of up to 131072 keys).
+// delivers the chunk's 64 KB.  What is left is the ring: shared memory holds Q (64 KB)
+// and 2.25 chunks, and a stage comes back only after its load (about 2000 cycles), its
+// chunk's softmax (1250) and both products, a period of 2850 to 3000 cycles.  Measured:
+// 5.5 TB/s (0.85 of the copy rate) between 40000 and 80000 keys of 16 rows, 5.0 TB/s
+// over whole calls (16 rows of 60000 keys: 193 us), of which about 17 us are start,
+// output and join.  Chunks of 128 keys cost fewer tensor cycles per key but hold all of
+// the ring until their softmax is done, and the loads stand still for half of the time
+// (16 rows of up to 131072 keys: 353 against 291 us at that step).
 //
 // Work split: the visible keys of all rows, in boxes of up to 64 keys on one page,
 // form one list, and the list is cut into equal shares, one per CTA (one CTA per

@@ -14,7 +14,12 @@
 // rotation runs in 32 bits with one rounding at the end.
 //
 // Both kernels are bound by HBM: every channel is read and written once (only
-// the rotated ones when x is rotated in place).
+// the rotated ones when x is rotated in place).  A thread has several units' loads in
+// flight before it waits for any (x may be y, so the compiler cannot do it), and ahead
+// of the angles.  Measured: 4099 tokens x 64 heads x 512 in bf16 (537 MB) 96 us, 5.6
+// TB/s, 0.86 of the copy rate (one unit at a time behind the angles: 155 us); 32771
+// cache rows (67 MB) 13.5 us, 5.0 TB/s; 64 rows 2.1 us, 64 tokens' queries 4.1 us,
+// which is launch and latency.
 #include <limits.h>
 #include <string.h>
 
