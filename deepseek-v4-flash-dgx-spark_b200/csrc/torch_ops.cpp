@@ -357,9 +357,12 @@ at::Tensor index_tensor(const at::Tensor& t, const at::Tensor& like, int64_t num
   return t.contiguous();
 }
 
+// A list of ids or lengths as int32; what does not fit becomes INT_MIN or INT_MAX, which
+// the kernels take as padding or refuse, instead of another sequence's id.
 at::Tensor int32_list(const at::Tensor& t, const at::Tensor& like, const char* name) {
   TORCH_CHECK(t.dim() == 1, name, " must have one dimension");
-  return index_tensor(t, like, t.numel(), name).to(at::kInt);
+  const at::Tensor v = index_tensor(t, like, t.numel(), name);
+  return v.scalar_type() == at::kInt ? v : v.clamp(INT32_MIN, INT32_MAX).to(at::kInt);
 }
 
 int rotated_channels(const at::Tensor& freqs, const at::Tensor& like) {
@@ -517,7 +520,7 @@ int* state_of(const at::Tensor& t, const at::Tensor& table, int64_t n, const cha
   return t.data_ptr<int>();
 }
 
-// seq_ids (optional) and positions as one index type.
+// seq_ids (optional) and positions as one index type, the wider where they differ.
 struct RowIndex {
   at::Tensor seqs, positions;
   bool is64;
@@ -526,11 +529,16 @@ struct RowIndex {
 RowIndex row_index(const OptT& seq_ids, const at::Tensor& positions, const at::Tensor& like, int64_t T, int n_seqs) {
   RowIndex r;
   r.positions = index_tensor(positions, like, T, "positions");
-  r.is64 = r.positions.scalar_type() == at::kLong;
-  if (seq_ids.has_value())
-    r.seqs = index_tensor(*seq_ids, like, T, "seq_ids").to(r.positions.scalar_type());
-  else
+  if (seq_ids.has_value()) {
+    r.seqs = index_tensor(*seq_ids, like, T, "seq_ids");
+    if (r.seqs.scalar_type() != r.positions.scalar_type()) {
+      r.seqs = r.seqs.to(at::kLong);
+      r.positions = r.positions.to(at::kLong);
+    }
+  } else {
     TORCH_CHECK(T <= n_seqs, "more rows than sequences: give seq_ids");
+  }
+  r.is64 = r.positions.scalar_type() == at::kLong;
   return r;
 }
 

@@ -66,7 +66,8 @@ def fork(pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, 
          parents: torch.Tensor, children: torch.Tensor, lens: torch.Tensor | None = None) -> None:
     """The empty sequence children[i] becomes the first lens[i] tokens (None: all)
     of parents[i].  Full pages are shared; a part-filled last page is copied to a
-    free page in every layer, so both may go on writing behind the fork."""
+    free page in every layer, so both may go on writing behind the fork (not before
+    it: those pages are the other's too)."""
     ops.load().cache_fork(pages, page_table, seq_lens, page_refs, parents, children, lens)
 
 

@@ -345,7 +345,7 @@ DSV4_API int dsv4_cache_free(int* page_table, int* seq_lens, int* page_refs, int
 /* fork: the empty sequence children[i] becomes the first fork_lens[i] tokens
  * (NULL: all) of parents[i].  Full pages are shared; a part-filled last page is
  * copied to a free page (lowest id first) in every layer, so either side may go
- * on writing behind the fork.  A child that holds tokens or is named again, or a
+ * on writing behind the fork (not before it: those pages are the other's too).  A child that holds tokens or is named again, or a
  * length beyond the parent's, is a bad entry; a negative id is padding; too few
  * free pages change nothing. */
 DSV4_API long long dsv4_cache_fork_workspace_bytes(int n, int n_seqs);

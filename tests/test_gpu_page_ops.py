@@ -106,6 +106,30 @@ def test_refused_entries_and_too_few_pages(cuda_device):
     c.reserve([5], [2 ** 31 - 1], bad=True)
 
 
+def test_64_bit_ids_do_not_wrap(cuda_device):
+    """2^32 is no sequence, not sequence 0; 2^32 + 5 no length of 5."""
+    from spark_b200 import _lib, kv_cache
+
+    c = Both(4, 4, 12, 16)
+    c.reserve([0, 1], [20, 30])
+    before = c.table.clone(), c.lens.clone(), c.refs.clone()
+    big = torch.tensor([2 ** 32, 2 ** 32 + 1], device="cuda")
+    small = torch.tensor([2, 3], device="cuda")
+    for call in (lambda: kv_cache.reserve(c.table, c.lens, c.refs, big, small, 16),
+                 lambda: kv_cache.reserve(c.table, c.lens, c.refs, small, big, 16),
+                 lambda: kv_cache.free(c.table, c.lens, c.refs, big),
+                 lambda: kv_cache.fork(c.pages, c.table, c.lens, c.refs, big, small),
+                 lambda: kv_cache.fork(c.pages, c.table, c.lens, c.refs, torch.tensor([0, 1], device="cuda"), big),
+                 lambda: kv_cache.copy_pages(c.pages, big, small)):
+        call()
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="cache sequence, position"):
+            _lib.raise_on_device_error()
+        assert torch.equal(c.table, before[0]) and torch.equal(c.lens, before[1]) and torch.equal(c.refs, before[2])
+    kv_cache.free(c.table, c.lens, c.refs, torch.tensor([-2 ** 40], device="cuda"))  # padding
+    c.same()
+
+
 def test_many_sequences_and_pages(cuda_device):
     rng = np.random.default_rng(5)
     c = Both(1500, 20, 20000, 16, layers=1, D=8)

@@ -270,6 +270,36 @@ def test_streams_and_graphs(cuda_device):
     _lib.raise_on_device_error()
 
 
+def test_raw_c_abi_and_mixed_index_types(cuda_device):
+    """The C entry with a caller's workspace gives the op's bytes; sequence ids and
+    positions of different widths are compared in the wider one."""
+    from spark_b200 import _lib, kv_cache
+
+    c = Cache([700, 33], 64, 512, torch.bfloat16, seed=9)
+    q = torch.randn(3, 64, 512, generator=c.g, device="cuda").bfloat16()
+    seq, pos = torch.tensor([1, 0, 0], device="cuda"), torch.tensor([32, 699, 5], device="cuda")
+    want = kv_cache.paged_attn(q, c.pages, c.table, seq, pos, None, 0.05)
+    lib = _lib.load()
+    need = int(lib.dsv4_paged_attn_workspace_bytes(3, 64, 512, 64, c.table.shape[1]))
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    _lib.check(lib.dsv4_paged_attn(q.data_ptr(), 64 * 512, 512, 0, 3, 64, 512, c.pages.data_ptr(), c.pages.shape[0], 64,
+                                   64 * 512, c.table.data_ptr(), 2, c.table.shape[1], seq.data_ptr(), pos.data_ptr(), 1,
+                                   None, 0.05, 0, 0, out.data_ptr(), ws.data_ptr(), need, _lib.stream_ptr()),
+               "dsv4_paged_attn")
+    assert torch.equal(out, want)
+    for s, p in ((seq.int(), pos), (seq, pos.int())):
+        assert torch.equal(kv_cache.paged_attn(q, c.pages, c.table, s, p, None, 0.05), want)
+    torch.cuda.synchronize()
+    _lib.raise_on_device_error()
+    wrapped = seq + torch.tensor([0, 2 ** 32, 0], device="cuda")
+    out = kv_cache.paged_attn(q, c.pages, c.table, wrapped, pos.int(), None, 0.05)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cache sequence, position"):
+        _lib.raise_on_device_error()
+    assert torch.all(out[1] == 0) and torch.equal(out[::2], want[::2])
+
+
 def test_argument_checks(cuda_device):
     from spark_b200 import kv_cache
 

@@ -126,6 +126,34 @@ def test_rotary_gradient(cuda_device):
     assert (gx - gg).abs().max().item() <= 2 * 4e-7 * 16
 
 
+def test_rotary_and_its_gradient_in_a_graph(cuda_device):
+    from spark_b200.rotary import rotary
+
+    f = _freqs(64)
+    x = torch.randn(3, 5, 2, 64, device="cuda", requires_grad=True)
+    w = torch.randn(3, 5, 2, 64, device="cuda")
+    pos = torch.randint(0, 1000, (3, 5), device="cuda")
+
+    def step():
+        y = rotary(x, pos, f)
+        return y.detach(), torch.autograd.grad(y, x, w)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, gx = step()
+    for p in (7, 99_000):
+        pos.fill_(p)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(y, x.detach(), pos, f, 0, True)
+        _check(gx, w, pos, f, 0, True, inverse=True)
+
+
 def test_rotary_refusals(cuda_device):
     from spark_b200.rotary import rotary, rotary_
 
