@@ -12,10 +12,10 @@
 // into a graph and need no copy of the tables on the host.
 //
 // The bookkeeping is a few hundred KB of integers and bound by latency: one CTA
-// of 1024 threads walks the page counts with ballots and one scan per 16384 pages (4096 in a small pool),
-// its results are the same in every run (free pages are taken in ascending order
-// and counts are integer sums), and the row copies follow as a second kernel over
-// all SMs, bound by HBM.  Measured: planning 4.5 us (1024 pages, fork or compact)
+// of 1024 threads walks the page counts with ballots and one scan per 16384 pages
+// (4096 in a small pool), its results are the same in every run (free pages are taken
+// in ascending order and counts are integer sums), and the row copies follow as a
+// second kernel over all SMs, bound by HBM.  Measured: planning 4.5 us (1024 pages, fork or compact)
 // and 11.6 us (255 sequences taking half of 32768 pages); the copies of a compaction
 // in 43 layers 166 us for about 1.08 GB, the rate of a plain copy.
 #include <limits.h>
@@ -100,7 +100,7 @@ __device__ __forceinline__ int collect_pages(const int* refs, int begin, int end
   return collect_step<16>(refs, begin, end, used, limit, list, scratch);
 }
 
-// Entry i's claim on sequence s: true for the first entry that names it.
+// owner[s] becomes the first entry that names sequence s (atomicMin over the entries).
 __device__ __forceinline__ void init_owners(int* owner, int n_seqs) {
   for (int s = threadIdx.x; s < n_seqs; s += blockDim.x) owner[s] = INT_MAX;
   __syncthreads();

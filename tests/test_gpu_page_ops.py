@@ -130,14 +130,25 @@ def test_64_bit_ids_do_not_wrap(cuda_device):
     c.same()
 
 
-def test_many_sequences_and_pages(cuda_device):
+@pytest.mark.parametrize("seqs", [1500, 2600])  # claims in shared memory, in the workspace
+def test_many_sequences_and_pages(cuda_device, seqs):
     rng = np.random.default_rng(5)
-    c = Both(1500, 20, 20000, 16, layers=1, D=8)
-    every = rng.permutation(1500).tolist()
-    c.reserve(every, rng.integers(0, 20 * 16 // 2, 1500).tolist())
+    c = Both(seqs, 20, 30000, 16, layers=1, D=8)
+    every = rng.permutation(seqs).tolist()
+    c.reserve(every, rng.integers(0, 20 * 16 // 2, seqs).tolist())
     c.free(every[:700])
-    c.reserve(every[:300], rng.integers(0, 20 * 16, 300).tolist())
+    c.reserve(every[:300] + every[:1], rng.integers(0, 20 * 16, 301).tolist(), bad=True)
     c.fork([every[0]] * 200 + every[701:900], every[300:699])
+    c.compact()
+    c.reserve(every, [160] * seqs)
+
+
+def test_few_long_sequences(cuda_device):
+    c = Both(5, 1500, 5000, 16, layers=1, D=8)
+    c.reserve([3, 1], [16 * 1400 + 3, 16 * 131])
+    c.reserve([0, 1, 4], [16 * 33, 16 * 700, 16 * 1500])
+    c.free([3])
+    c.fork([4, 1], [2, 3])
     c.compact()
 
 

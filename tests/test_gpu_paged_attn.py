@@ -142,6 +142,25 @@ def test_rows_of_one_sequence_padding_and_order(cuda_device):
     _check(out, q, lambda t, keys: c.rows[0][keys], list(range(300)), None, 0.05, 0, 0)
 
 
+@pytest.mark.parametrize("H,window", [(16, 0), (100, 60)])
+def test_more_rows_than_threads(cuda_device, H, window):
+    """Several rows per thread where the shares are worked out, padding among them, and
+    rows of two head groups."""
+    from spark_b200 import _lib, kv_cache
+
+    c = Cache([300, 1, 77, 200], 16, 128, torch.bfloat16, seed=12)
+    rng = np.random.default_rng(1)
+    seq = rng.integers(-1, 4, 900)
+    pos = np.array([-1 if s < 0 else int(rng.integers(0, len(c.rows[s]))) for s in seq])
+    q = torch.randn(900, H, 128, generator=c.g, device="cuda").bfloat16()
+    out = kv_cache.paged_attn(q, c.pages, c.table, torch.from_numpy(seq).cuda(), torch.from_numpy(pos).cuda(), None, 0.1,
+                              window=window)
+    torch.cuda.synchronize()
+    _lib.raise_on_device_error()
+    _check(out, q, lambda t, keys: c.rows[seq[t]][keys], pos.tolist(), None, 0.1, window, 0)
+    assert torch.all(out[torch.from_numpy(pos < 0).cuda()] == 0)
+
+
 def test_missing_pages_are_left_out_and_reported(cuda_device):
     from spark_b200 import _lib, kv_cache
 
