@@ -7,7 +7,8 @@
 // Row t stands at position p of sequence s and sees the keys j <= p, with a
 // window only those above p - window and the first `first` ones.  Key j is row
 // j % page_size of page page_table[s][j / page_size]; one cache row is key and
-// value of every head.  A row with nothing visible gives zeros.
+// value of every head.  A row with nothing visible gives zeros; scores of NaN or
+// infinities give what the formula does, whether one CTA holds the row or several.
 //
 // Per chunk of 64 keys two products on tcgen05 (kind::f16, fp32 accumulators in TMEM):
 //   S[h,j]   = Q[h,:] . C[j,:]      M = 64 heads, N = 64 keys, K = D
@@ -64,7 +65,7 @@ constexpr int kPaTmemCols = 512;                  // S: two buffers of 64 column
 constexpr int kPaMinChunks = 1;                   // least chunks per CTA
 constexpr int kPaSnapChunks = 3;                  // a border moves so far to a row's begin or end
 constexpr float kPaRescaleLog2 = 10.0f;           // headroom of the running max, base 2
-constexpr float kPaNoMax = -3.402823466e38f;      // running max of a piece before its first key
+constexpr float kPaNoMax = -3.402823466e38f;      // running max of a piece before its first finite score
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct PaArgs {
@@ -74,7 +75,7 @@ struct PaArgs {
   const void* positions;  // [T]
   const float* sink;      // [H] or NULL
   float* part_o;          // [grid][2][N][D]
-  float* part_ml;         // [grid][2][N][2]: max (base 2), sum
+  float* part_ml;         // [grid][2][N][2]: max (base 2; -inf: no key seen), sum
   int4* plan;             // [grid]: row, head group, boxes of the row before this CTA's border, boxes of the row
   int* share;             // [1] boxes from border to border
   int T, H, D, groups;
@@ -643,9 +644,11 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           return false;
         };
         float m_a = kPaNoMax, m_b = kPaNoMax, l_a = 0.f, l_b = 0.f;
+        bool any_seen = false;  // of the piece's keys
         bool see0 = seen(i, lane), see1 = seen(i, lane + 32);
         for (; i < i1; i += nsub, ++k) {
           const uint32_t lo = __ballot_sync(0xffffffffu, see0), hi = __ballot_sync(0xffffffffu, see1);
+          any_seen |= (lo | hi) != 0;
           if (i + nsub < i1) {
             see0 = seen(i + nsub, lane);
             see1 = seen(i + nsub, lane + 32);
@@ -762,8 +765,9 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             sh.red[64 * half + ha] = l_a;
             sh.red[64 * half + ha + 8] = l_b;
             if (half == 0) {
-              sh.m[ha] = m_a;
-              sh.m[ha + 8] = m_b;
+              // no key at all is told apart from scores that raised no max (NaN, -inf)
+              sh.m[ha] = any_seen ? m_a : -INFINITY;
+              sh.m[ha + 8] = any_seen ? m_b : -INFINITY;
             }
           }
         }
@@ -779,7 +783,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             const float sk = a.sink && st < heads ? __ldg(a.sink + 64 * g + st) * kLog2e : -INFINITY;
             const float mx = fmaxf(m, sk);
             const float den = l * ex2(m - mx) + pa_sink(sk, mx);
-            sh.f[st] = m == kPaNoMax ? 0.f : ex2(m - mx) / den;
+            sh.f[st] = m == -INFINITY ? 0.f : ex2(m - mx) / den;
           } else {
             a.part_ml[(piece * N + st) * 2] = m;
             a.part_ml[(piece * N + st) * 2 + 1] = l;
@@ -897,17 +901,20 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaA
       }
     };
     load(p0);  // on the way while the maxima are compared
-    float mx = sk;
-    for (int i = lane; i < r.w; i += 32) mx = fmaxf(mx, a.part_ml[piece(i) * 2]);
+    float top = -INFINITY;
+    for (int i = lane; i < r.w; i += 32) top = fmaxf(top, a.part_ml[piece(i) * 2]);
 #pragma unroll
-    for (int x = 16; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const bool any_seen = top > -INFINITY;
+    const float mx = fmaxf(top, sk);
     float den = 0.f;
     float4 acc[4] = {};
     for (int i0 = p0; i0 < r.w; i0 += ps * kJoinAhead) {
       if (i0 != p0) load(i0);
 #pragma unroll
       for (int j = 0; j < kJoinAhead; ++j) {
-        if (i0 + j * ps >= r.w || ml[j].x == kPaNoMax) continue;
+        // only a piece that saw no key is left out: NaN and infinities reach the sum
+        if (i0 + j * ps >= r.w || ml[j].x == -INFINITY) continue;
         const float f = ex2(ml[j].x - mx);
         den += ml[j].y * f;
 #pragma unroll
@@ -941,9 +948,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PaA
       }
       acc[0] = sum;
     }
-    const bool any = den != 0.f;
     den += pa_sink(sk, mx);
-    const float inv = any ? 1.f / den : 0.f;
+    const float inv = any_seen ? 1.f / den : 0.f;
     T* dst = static_cast<T*>(a.out) + ((size_t)r.x * a.H + head) * a.D + (together ? 128 * warp : 0) + 4 * lane;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {

@@ -1,0 +1,112 @@
+"""Paged attention on values that are no ordinary numbers: NaN and infinities in
+queries, keys and sinks, and pages that are missing, in rows that one block holds
+whole and in rows joined from pieces.  The formula in float64 says where NaN belongs
+(oracle/cache_oracle.py ``paged_attn``); everything else obeys its bound."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache_oracle as C
+from test_gpu_paged_attn import HALF, TINY, Cache
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+LENS = [40, 3000, 64, 9001]  # whole, joined, whole, joined
+
+
+def _check(out, q, kv_of, pos, sink, scale):
+    with np.errstate(all="ignore"):
+        ref, bound = C.paged_attn(q.double().cpu().numpy(), kv_of, pos, None if sink is None else sink.cpu().numpy(),
+                                  scale, 0, 0, HALF[q.dtype], TINY[q.dtype])
+    got = out.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(ref))
+    there = ~np.isnan(ref)
+    assert np.all(np.abs(got - ref)[there] <= bound[there])
+
+
+def _put(c, t, first, last, channel, value):
+    """``value`` into one channel of keys first .. last - 1 of sequence t."""
+    for j in range(first, last):
+        c.pages[c.table[t, j // c.page].long(), j % c.page, channel] = value
+    c.rows[t][first:last, channel] = value
+
+
+def _attend(c, H, dtype, sink, change_q=None):
+    from spark_b200 import kv_cache
+
+    D = c.pages.shape[2]
+    q = torch.randn(len(LENS), H, D, generator=c.g, device="cuda").to(dtype)
+    if change_q is not None:
+        change_q(q)
+    s = torch.randn(H, generator=c.g, device="cuda") if sink else None
+    pos = [n - 1 for n in LENS]
+    out = kv_cache.paged_attn(q, c.pages, c.table, None, torch.tensor(pos, device="cuda"), s, D ** -0.5)
+    torch.cuda.synchronize()
+    _check(out, q, lambda t, keys: c.rows[t][keys], pos, s, D ** -0.5)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,sink", [(64, True), (16, False)])
+def test_nan_in_a_query(cuda_device, dtype, H, sink):
+    """One head of every row has a NaN: all its scores are NaN, so is its output, whole
+    or joined; the other heads are as they would be."""
+    from spark_b200 import _lib
+
+    def change(q):
+        q[:, 3, 5] = NAN
+
+    out = _attend(Cache(LENS, 64, 128, dtype, seed=H), H, dtype, sink, change)
+    _lib.raise_on_device_error()
+    assert torch.isnan(out[:, 3]).all() and torch.isfinite(out[:, 4:]).all()
+
+
+@pytest.mark.parametrize("sink", [True, False])
+@pytest.mark.parametrize("t,first,last", [(0, 0, 40), (1, 64, 128), (1, 0, 3000), (2, 63, 64), (3, 0, 1), (3, 4480, 4736),
+                                          (3, 8960, 9001)])
+def test_pages_of_nan(cuda_device, t, first, last, sink):
+    c = Cache(LENS, 64, 512, torch.bfloat16, seed=first)
+    _put(c, t, first, last, slice(None), NAN)
+    out = _attend(c, 64, torch.bfloat16, sink)
+    assert torch.isnan(out[t]).all()
+    assert torch.isfinite(out[[x for x in range(4) if x != t]]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sink", [True, False])
+@pytest.mark.parametrize("value", [INF, -INF])
+@pytest.mark.parametrize("t,first,last", [(0, 7, 8), (0, 0, 40), (1, 64, 128), (1, 0, 3000), (2, 0, 64), (3, 4000, 5000),
+                                          (3, 0, 9001)])
+def test_infinite_keys(cuda_device, dtype, t, first, last, value, sink):
+    """A score of +inf makes its head NaN; one of -inf has weight 0, and 0 x inf is NaN
+    in the infinite channel.  Where every score is -inf the weights are 0 / 0, unless
+    a sink keeps the denominator."""
+    c = Cache(LENS, 64, 128, dtype, seed=last)
+    _put(c, t, first, last, 9, value)
+    out = _attend(c, 16, dtype, sink)
+    assert torch.isnan(out[t, :, 9]).all() and torch.isfinite(out[[x for x in range(4) if x != t]]).all()
+
+
+@pytest.mark.parametrize("sink", [None, 0.5, INF])
+def test_rows_on_no_page_give_zeros(cuda_device, sink):
+    """Nothing seen is told apart from scores of -inf: zeros and a latched error, whole or
+    joined, also where only some pieces see nothing."""
+    from spark_b200 import _lib, kv_cache
+
+    c = Cache(LENS, 64, 128, torch.bfloat16, seed=2)
+    c.table[0], c.table[1], c.table[3, 8:100] = -1, -1, -1
+    q = torch.randn(len(LENS), 16, 128, generator=c.g, device="cuda").bfloat16()
+    s = None if sink is None else torch.full((16,), sink, device="cuda")
+    pos = [n - 1 for n in LENS]
+    out = kv_cache.paged_attn(q, c.pages, c.table, None, torch.tensor(pos, device="cuda"), s, 0.1)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cache sequence, position"):
+        _lib.raise_on_device_error()
+    assert torch.all(out[:2] == 0)
+    if sink != INF:
+        _check(out[2:], q[2:], lambda t, keys: c.rows[2 + t][keys if t == 0 else keys[(keys < 512) | (keys >= 6400)]],
+               [63, 9000], s, 0.1)
+    else:
+        assert torch.all(out == 0)
