@@ -142,15 +142,17 @@ def visible(position: int, window: int, first: int) -> np.ndarray:
     return keys if not window else keys[(keys > position - window) | (keys < first)]
 
 
-def paged_attn(q, kv_of, positions, sink, scale, window=0, first=0, half_step=0.0, tiny=0.0):
+def paged_attn(q, kv_of, positions, sink, scale, window=0, first=0, half_step=0.0, tiny=0.0, weight_tiny=None):
     """q [T,H,D]; kv_of(t, keys) -> rows of row t's sequence; positions [T] (negative:
     padding).  Returns float64 out [T,H,D] and the largest error of a kernel that rounds
     the weights p and the output to a type with the given half step (relative):
 
     with weights p_j (1 + d_j), |d_j| <= half_step, summed as rounded, the quotient is off
     by at most half_step (sum p|kv| + |out|) to first order, its rounding by another
-    half_step |out|; weights below the type's normal range are off by tiny / 2 each (the
-    largest weight is at least 1 before the division).  Scores and exponentials in 32
+    half_step |out|; weights below the type's normal range are off by weight_tiny / 2 of the
+    largest weight each (default: tiny, where the largest weight is at least 1 before the
+    division; tiny / 2^k where it is at least 2^k).  That term grows with the number of
+    keys: without a k it hides the loss of many small weights.  Scores and exponentials in 32
     bits add a relative 1e-4 at most (|z| < 100, 512 products: 512 2^-24 times
     scale sum |q k| < 30, and 2^-22 |z|), taken as 3e-4 of sum p|kv| + |out|."""
     q = np.asarray(q, np.float64)
@@ -172,6 +174,6 @@ def paged_attn(q, kv_of, positions, sink, scale, window=0, first=0, half_step=0.
         out[t] = p @ kv
         spread = p @ np.abs(kv) + np.abs(out[t])
         largest = np.exp(top - m) / den
-        small = tiny / 2 * largest[:, None] * np.abs(kv).sum(0)[None]
+        small = (tiny if weight_tiny is None else weight_tiny) / 2 * largest[:, None] * np.abs(kv).sum(0)[None]
         bound[t] = (1.02 * half_step + 3e-4) * spread + half_step * np.abs(out[t]) + small + tiny / 2
     return out, bound

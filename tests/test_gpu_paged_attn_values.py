@@ -110,3 +110,62 @@ def test_rows_on_no_page_give_zeros(cuda_device, sink):
                [63, 9000], s, 0.1)
     else:
         assert torch.all(out == 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nats,small", [(18, 1e-3), (22, 1e-4)])
+@pytest.mark.parametrize("place", [0, 2050, 4000])
+def test_a_dominating_key_of_small_values(cuda_device, dtype, nats, small, place):
+    """One key far above thousands of others, with values so small that the others' tiny
+    weights still make a part of the output.  In fp16 the largest weight is at least 2^9
+    and the steps are 2^-24: a key loses 2^-34 of the largest weight at most."""
+    from spark_b200 import _lib, kv_cache
+
+    T, H, D, n = 300, 3, 128, 4001
+    c = Cache([n], 64, D, dtype, seed=place)
+    rows = torch.randn(n, D, generator=c.g, device="cuda") + 1.0
+    rows[place] *= small
+    rows[:, 0] = 0.0
+    rows[place, 0] = 1.0
+    rows = rows.to(dtype)
+    for j in range(-(-n // 64)):
+        part = rows[j * 64:(j + 1) * 64]
+        c.pages[c.table[0, j].long(), : len(part)] = part
+    q = torch.zeros(T, H, D, device="cuda")
+    q[:, :, 0] = torch.tensor([nats, nats - 3.0, 1.0], device="cuda")
+    q = q.to(dtype)
+    pos = [n - 1 - (t % 3) if place < 4000 else n - 1 for t in range(T)]
+    out = kv_cache.paged_attn(q, c.pages, c.table, torch.zeros(T, dtype=torch.int32, device="cuda"),
+                              torch.tensor(pos, dtype=torch.int32, device="cuda"), None, 1.0)
+    torch.cuda.synchronize()
+    _lib.raise_on_device_error()
+    kv = rows.double().cpu().numpy()
+    ref, bound = C.paged_attn(q.double().cpu().numpy(), lambda t, keys: kv[keys], pos, None, 1.0, 0, 0, HALF[dtype],
+                              TINY[dtype], TINY[dtype] * 2.0 ** -9)
+    err = np.abs(out.double().cpu().numpy() - ref)
+    assert np.all(err <= bound), (float((err / bound).max()), float(err.max()))
+
+
+def test_rising_scores_in_fp16(cuda_device):
+    """Scores that rise by two to forty in base 2 from chunk to chunk, and fall again: no
+    weight passes fp16's range."""
+    from spark_b200 import _lib, kv_cache
+
+    D, H, n = 128, 64, 2500
+    c = Cache([n, n], 64, D, torch.float16, seed=1)
+    q = torch.zeros(2, H, D, device="cuda").half()
+    q[:, :, 0] = torch.linspace(-20, 20, H, device="cuda").half()
+    rows = torch.from_numpy(c.rows[0]).cuda()
+    rows[:, 0] = torch.cat((torch.linspace(0, 30, 1500), torch.linspace(30, -30, 1000))).half().double().cuda()
+    for t in range(2):
+        for j in range(-(-n // 64)):
+            part = rows[j * 64:(j + 1) * 64]
+            c.pages[c.table[t, j].long(), : len(part)] = part.half()
+    kv = rows.cpu().numpy()
+    out = kv_cache.paged_attn(q, c.pages, c.table, None, torch.tensor([n - 1, 63], device="cuda"), None, 1.0)
+    torch.cuda.synchronize()
+    _lib.raise_on_device_error()
+    ref, bound = C.paged_attn(q.double().cpu().numpy(), lambda t, keys: kv[keys], [n - 1, 63], None, 1.0, 0, 0,
+                              HALF[torch.float16], TINY[torch.float16], TINY[torch.float16] * 2.0 ** -9)
+    err = np.abs(out.double().cpu().numpy() - ref)
+    assert np.all(err <= bound), (float((err / bound).max()), float(err.max()))
