@@ -283,6 +283,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return (uint32_t)x | ((uint32_t)y << 16);
 }
 
+// The sum of two packed values in 32 bits.
+template <typename T>
+__device__ __forceinline__ float sum2(uint32_t v) {
+  if constexpr (std::is_same<T, __half>::value) {
+    __half2 h;
+    memcpy(&h, &v, 4);
+    const float2 f = __half22float2(h);
+    return f.x + f.y;
+  } else {
+    return __uint_as_float(v << 16) + __uint_as_float(v & 0xffff0000u);
+  }
+}
+
 // Lane l of four holds column l of four rows; it gets row l % 4 of the four columns.
 __device__ __forceinline__ float4 transpose4(float a0, float a1, float a2, float a3, int lane) {
   const bool o1 = lane & 1, o2 = lane & 2;
@@ -750,18 +763,18 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             }
           }
           if (active) {
-            // weights, rounded to the cache's type as the product takes them; the sum adds
-            // them unrounded (their rounding errors average out over the keys)
+            // weights, rounded to the cache's type as the product takes them, and summed as
+            // rounded: the error of a weight that dominates its row then cancels in the quotient
             uint8_t* p0 = sP + b * (N * 128) + ha * 128 + 4 * (lane & 3);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const float e0 = ex2(z[4 * c] - m_a), e1 = ex2(z[4 * c + 1] - m_a);
-              const float e2 = ex2(z[4 * c + 2] - m_b), e3 = ex2(z[4 * c + 3] - m_b);
-              l_a += e0 + e1;
-              l_b += e2 + e3;
+              const uint32_t w_a = pack2<T>(ex2(z[4 * c] - m_a), ex2(z[4 * c + 1] - m_a));
+              const uint32_t w_b = pack2<T>(ex2(z[4 * c + 2] - m_b), ex2(z[4 * c + 3] - m_b));
+              l_a += sum2<T>(w_a);
+              l_b += sum2<T>(w_b);
               const int unit = ((4 * half + c) ^ (ha & 7)) << 4;  // rows ha and ha + 8 swizzle alike
-              *reinterpret_cast<uint32_t*>(p0 + unit) = pack2<T>(e0, e1);
-              *reinterpret_cast<uint32_t*>(p0 + 8 * 128 + unit) = pack2<T>(e2, e3);
+              *reinterpret_cast<uint32_t*>(p0 + unit) = w_a;
+              *reinterpret_cast<uint32_t*>(p0 + 8 * 128 + unit) = w_b;
             }
           }
           fence_proxy_async_shared();

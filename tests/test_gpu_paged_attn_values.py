@@ -169,3 +169,40 @@ def test_rising_scores_in_fp16(cuda_device):
                               HALF[torch.float16], TINY[torch.float16], TINY[torch.float16] * 2.0 ** -9)
     err = np.abs(out.double().cpu().numpy() - ref)
     assert np.all(err <= bound), (float((err / bound).max()), float(err.max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [200, 2000])
+def test_the_error_of_a_dominating_weight_cancels(cuda_device, dtype, n):
+    """A key that takes nearly all of the weight, behind the one that set the running max,
+    so that its own weight is no power of two (as many rows as leave each to one block).  Weights p_j (1 + d_j) summed as rounded
+    give sum p_j (1 + d_j) kv_j / sum p_j (1 + d_j) = out + sum d_j p_j (kv_j - out) to
+    first order: half a step of sum p_j |kv_j - out|, not of sum p_j |kv_j|, then the
+    output's half step and 3e-4 of sum p |kv| + |out| for scores and exponentials in
+    32 bits (cache_oracle.paged_attn)."""
+    from spark_b200 import _lib, kv_cache
+
+    D, H = 128, 64
+    c = Cache([n], 64, D, dtype, seed=n)
+    rows = torch.randn(n, D, generator=c.g, device="cuda")
+    rows[:, 0], rows[0, 0], rows[150, 0] = -5.0, 0.0, 1.0
+    rows = rows.to(dtype)
+    for j in range(-(-n // 64)):
+        part = rows[j * 64:(j + 1) * 64]
+        c.pages[c.table[0, j].long(), : len(part)] = part
+    q = torch.zeros(300, H, D, device="cuda")
+    q[:, :, 0] = torch.linspace(3, 4, H, device="cuda")
+    q = q.to(dtype)
+    where = torch.zeros(300, dtype=torch.int32, device="cuda"), torch.full((300,), n - 1, dtype=torch.int32, device="cuda")
+    out = kv_cache.paged_attn(q, c.pages, c.table, *where, None, 1.0)
+    torch.cuda.synchronize()
+    _lib.raise_on_device_error()
+    kv = rows.double().cpu().numpy()
+    z = q[0].double().cpu().numpy() @ kv.T
+    p = np.exp(z - z.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    ref = p @ kv
+    apart = np.stack([p[h] @ np.abs(kv - ref[h]) for h in range(H)])
+    bound = 1.02 * HALF[dtype] * apart + HALF[dtype] * np.abs(ref) + 3e-4 * (p @ np.abs(kv) + np.abs(ref)) + TINY[dtype]
+    err = np.abs(out.double().cpu().numpy() - ref)
+    assert np.all(err <= bound), (float((err / bound).max()), int((err > bound).sum()))
