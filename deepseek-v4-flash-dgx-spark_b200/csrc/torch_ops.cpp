@@ -453,6 +453,11 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
 
 at::Tensor rotary_autograd(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
                            std::optional<int64_t> offset, bool inverse, double amplitude) {
+  if (x._fw_grad(0).defined()) {  // forward mode: the map is linear, the tangent turns with x
+    const auto [primal, tangent] = at::_unpack_dual(x, 0);
+    return at::_make_dual(call_rotary(primal, positions, freqs, interleaved, offset, inverse, amplitude),
+                          call_rotary(tangent, positions, freqs, interleaved, offset, inverse, amplitude), 0);
+  }
   if (at::GradMode::is_enabled() && x.requires_grad())
     return RotaryFunction::apply(x, positions, freqs, interleaved, offset, inverse, amplitude);
   at::AutoDispatchBelowADInplaceOrView below;

@@ -3,7 +3,8 @@
 * ``rotary_frequencies(rot, ...)``: radians per position of each channel pair,
   plain, linearly stretched or stretched by wavelength ("yarn"), in float64;
   made once and kept.
-* ``rotary(x, positions, freqs, ...)``: the rotated copy, with a gradient.
+* ``rotary(x, positions, freqs, ...)``: the rotated copy, differentiable in x in
+  backward and forward mode.
 * ``rotary_(x, positions, freqs, ...)``: in place, touching the rotated
   channels only; what a serving loop calls on its queries and, with
   ``inverse=True``, on the attention's output.
