@@ -26,6 +26,8 @@
 #include <cstring>
 #include <optional>
 #include <string>
+#include <tuple>
+#include <utility>
 #include <vector>
 
 #include "dsv4moe.h"
@@ -865,6 +867,43 @@ int64_t read_into(int64_t fd, at::Tensor& destination, int64_t size, int64_t off
   return got;
 }
 
+// The operators that write into their first `kWritten` arguments: those get a new version,
+// so that a backward pass which saved one of them is refused.
+template <typename Tuple, size_t... i>
+void bump_versions(const Tuple& args, std::index_sequence<i...>) {
+  (torch::autograd::impl::bump_version(std::get<i>(args)), ...);
+}
+
+template <const char* kName, size_t kWritten, typename F>
+struct Writing;
+template <const char* kName, size_t kWritten, typename R, typename... A>
+struct Writing<kName, kWritten, R(A...)> {
+  static R versioned(A... args) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow(kName, "").template typed<R(A...)>();
+    const auto bump = [&] { bump_versions(std::tie(args...), std::make_index_sequence<kWritten>()); };
+    at::AutoDispatchBelowADInplaceOrView below;
+    if constexpr (std::is_void_v<R>) {
+      op.call(args...);
+      bump();
+    } else {
+      R r = op.call(args...);
+      bump();
+      return r;
+    }
+  }
+};
+
+#define DSV4_WRITING(name, n)                      \
+  constexpr char k_##name[] = "dsv4moe::" #name;   \
+  using Writing_##name = Writing<k_##name, n, decltype(name)>
+DSV4_WRITING(rotary_, 1);
+DSV4_WRITING(cache_append, 1);
+DSV4_WRITING(cache_reserve, 3);
+DSV4_WRITING(cache_free, 3);
+DSV4_WRITING(cache_fork, 4);
+DSV4_WRITING(cache_compact, 3);
+DSV4_WRITING(cache_copy, 1);
+
 }  // namespace
 
 #define DSV4_LAYER_ARGS "Tensor?[] layer, int[] dims, float[] scalars"
@@ -954,6 +993,16 @@ TORCH_LIBRARY_IMPL(dsv4moe, CUDA, m) {
   m.impl("cache_compact", &cache_compact);
   m.impl("cache_copy", &cache_copy);
   m.impl("paged_attn", &paged_attn);
+}
+
+TORCH_LIBRARY_IMPL(dsv4moe, ADInplaceOrView, m) {
+  m.impl("rotary_", &Writing_rotary_::versioned);
+  m.impl("cache_append", &Writing_cache_append::versioned);
+  m.impl("cache_reserve", &Writing_cache_reserve::versioned);
+  m.impl("cache_free", &Writing_cache_free::versioned);
+  m.impl("cache_fork", &Writing_cache_fork::versioned);
+  m.impl("cache_compact", &Writing_cache_compact::versioned);
+  m.impl("cache_copy", &Writing_cache_copy::versioned);
 }
 
 TORCH_LIBRARY_IMPL(dsv4moe, Autograd, m) {

@@ -32,3 +32,56 @@ def test_rotary_has_a_tangent(dsv4):
         assert fw.unpack_dual(dsv4.rotary(x, pos, f)).tangent is None
     y, t = torch.func.jvp(lambda v: dsv4.rotary(v, pos, f), (x.detach(),), (torch.empty_like(x).detach(),))
     assert y.shape == t.shape == x.shape
+
+
+def _calls(op):
+    """Every operator that writes: the call, and the tensors it writes."""
+    def ints(*shape):
+        return torch.empty(*shape, dtype=torch.int32, device=META)
+
+    def bf16(*shape):
+        return torch.empty(*shape, dtype=torch.bfloat16, device=META)
+
+    x, pos, f = _rotary_args()
+    pages, table, lens, refs, ids = bf16(2, 9, 16, 64), ints(4, 8), ints(4), ints(9), ints(2)
+    rows, f16 = bf16(2, 64), torch.empty(16, dtype=torch.float64, device=META)
+    layer = pages[0]
+    return {
+        "rotary_": (lambda: op.rotary_(x, pos, f), [x]),
+        "cache_append": (lambda: op.cache_append(layer, rows, table, ids, ids, f16), [pages]),
+        "cache_reserve": (lambda: op.cache_reserve(table, lens, refs, ids, ids, 16), [table, lens, refs]),
+        "cache_free": (lambda: op.cache_free(table, lens, refs, ids), [table, lens, refs]),
+        "cache_fork": (lambda: op.cache_fork(pages, table, lens, refs, ids, ids), [pages, table, lens, refs]),
+        "cache_compact": (lambda: op.cache_compact(pages, table, refs), [pages, table, refs]),
+        "cache_copy": (lambda: op.cache_copy(pages, ids, ids), [pages]),
+    }
+
+
+WRITING = ["rotary_", "cache_append", "cache_reserve", "cache_free", "cache_fork", "cache_compact", "cache_copy"]
+
+
+@pytest.mark.parametrize("name", WRITING)
+def test_what_is_written_gets_a_new_version(dsv4, name):
+    """Also through a view (a layer of the pages), under no_grad and in inference mode, as
+    torch's own in-place operators do; what is only read keeps its version."""
+    call, written = _calls(dsv4)[name]
+    for mode in (torch.enable_grad, torch.no_grad, torch.inference_mode):
+        before = [t._version for t in written]
+        with mode():
+            call()
+        assert [t._version for t in written] == [v + 1 for v in before]
+    with torch.inference_mode():
+        _calls(dsv4)[name][0]()  # on inference tensors, which have no version
+
+
+def test_a_tensor_turned_in_place_is_refused_by_an_earlier_backward(dsv4):
+    x, pos, f = _rotary_args()
+    w = torch.empty_like(x, requires_grad=True)
+    z = (x * w).sum()
+    dsv4.rotary_(x, pos, f)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    y = dsv4.rotary(w, pos, f).sum()
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
