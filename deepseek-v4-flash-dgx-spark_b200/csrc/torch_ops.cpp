@@ -455,6 +455,8 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
 
 at::Tensor rotary_autograd(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
                            std::optional<int64_t> offset, bool inverse, double amplitude) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && freqs.requires_grad()) && !freqs._fw_grad(0).defined(),
+              "rotary has no gradient of freqs");
   if (x._fw_grad(0).defined()) {  // forward mode: the map is linear, the tangent turns with x
     const auto [primal, tangent] = at::_unpack_dual(x, 0);
     return at::_make_dual(call_rotary(primal, positions, freqs, interleaved, offset, inverse, amplitude),
@@ -469,7 +471,6 @@ at::Tensor rotary_autograd(const at::Tensor& x, const at::Tensor& positions, con
 void rotary_(at::Tensor x, const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
              std::optional<int64_t> offset, bool inverse, double amplitude) {
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
-  TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), "rotary_ has no gradient: use rotary");
   TORCH_CHECK(at::has_internal_overlap(x) != at::MemOverlap::Yes, "x must not overlap itself (expanded tensor)");
   const at::Tensor v = four_dims(x, false);
   run_rotary(v, v, positions, freqs, interleaved, offset, inverse, amplitude);
@@ -893,9 +894,35 @@ struct Writing<kName, kWritten, R(A...)> {
   }
 };
 
-#define DSV4_WRITING(name, n)                      \
-  constexpr char k_##name[] = "dsv4moe::" #name;   \
-  using Writing_##name = Writing<k_##name, n, decltype(name)>
+// The operators that have no derivative refuse tensors that want one, instead of dropping it.
+void refuse_gradient(const char* op, const at::Tensor& t) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined(), op,
+              " has no gradient, but an argument requires one: call it under torch.no_grad(), or detach the argument");
+}
+void refuse_gradient(const char* op, const OptT& t) {
+  if (t.has_value() && t->defined()) refuse_gradient(op, *t);
+}
+template <typename T>
+void refuse_gradient(const char*, const T&) {}
+
+template <const char* kName, typename F>
+struct NoGradient;
+template <const char* kName, typename R, typename... A>
+struct NoGradient<kName, R(A...)> {
+  static R checked(A... args) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow(kName, "").template typed<R(A...)>();
+    (refuse_gradient(kName, args), ...);
+    at::AutoDispatchBelowAutograd below;
+    return op.call(args...);
+  }
+};
+
+constexpr char k_paged_attn[] = "dsv4moe::paged_attn";
+using NoGradient_paged_attn = NoGradient<k_paged_attn, decltype(paged_attn)>;
+#define DSV4_WRITING(name, n)                                  \
+  constexpr char k_##name[] = "dsv4moe::" #name;               \
+  using Writing_##name = Writing<k_##name, n, decltype(name)>; \
+  using NoGradient_##name = NoGradient<k_##name, decltype(name)>
 DSV4_WRITING(rotary_, 1);
 DSV4_WRITING(cache_append, 1);
 DSV4_WRITING(cache_reserve, 3);
@@ -1007,6 +1034,14 @@ TORCH_LIBRARY_IMPL(dsv4moe, ADInplaceOrView, m) {
 
 TORCH_LIBRARY_IMPL(dsv4moe, Autograd, m) {
   m.impl("rotary", &rotary_autograd);
+  m.impl("rotary_", &NoGradient_rotary_::checked);
+  m.impl("cache_append", &NoGradient_cache_append::checked);
+  m.impl("cache_reserve", &NoGradient_cache_reserve::checked);
+  m.impl("cache_free", &NoGradient_cache_free::checked);
+  m.impl("cache_fork", &NoGradient_cache_fork::checked);
+  m.impl("cache_compact", &NoGradient_cache_compact::checked);
+  m.impl("cache_copy", &NoGradient_cache_copy::checked);
+  m.impl("paged_attn", &NoGradient_paged_attn::checked);
 }
 
 // Ops without tensor inputs on a device (sizes, host reads) dispatch here.

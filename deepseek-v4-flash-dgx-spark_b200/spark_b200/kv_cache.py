@@ -14,6 +14,8 @@ changes the tables in stream order without reading anything back, so a decode
 step (reserve, append, attend) can be captured into a CUDA graph.  Entries that
 make no sense (ids out of range, no page at a position, too few free pages) are
 skipped and latch a device-side error, read by ``_lib.raise_on_device_error()``.
+None of them has a gradient: tensors that require one are refused, except under
+``torch.no_grad()`` or in inference mode.
 
 ``PagedKVCache`` holds the tensors and calls the functions.
 """

@@ -85,3 +85,45 @@ def test_a_tensor_turned_in_place_is_refused_by_an_earlier_backward(dsv4):
     pos.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def _attn_args():
+    return {"q": torch.empty(3, 16, 128, dtype=torch.bfloat16, device=META),
+            "pages": torch.empty(9, 16, 128, dtype=torch.bfloat16, device=META),
+            "table": torch.empty(4, 8, dtype=torch.int32, device=META),
+            "seq": torch.empty(3, dtype=torch.int32, device=META), "pos": torch.empty(3, dtype=torch.int32, device=META),
+            "sink": torch.empty(16, device=META)}
+
+
+def _refused(call, tensors):
+    """Refused where one of the tensors requires a gradient or has a tangent; not under
+    no_grad, nor where none does."""
+    call(tensors)
+    for name, t in tensors.items():
+        if not t.is_floating_point():
+            continue
+        needs = dict(tensors, **{name: t.clone().requires_grad_()})
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(needs)
+        with torch.no_grad():
+            call(needs)
+        with fw.dual_level():
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="no gradient"):
+                    call(dict(tensors, **{name: fw.make_dual(t.clone(), torch.empty_like(t))}))
+
+
+def test_operators_without_a_gradient_refuse_one(dsv4):
+    _refused(lambda a: dsv4.paged_attn(a["q"], a["pages"], a["table"], a["seq"], a["pos"], a["sink"], 0.1), _attn_args())
+    a = _attn_args()
+    a["rows"], a["f"] = torch.empty(3, 128, dtype=torch.bfloat16, device=META), torch.empty(32, dtype=torch.float64, device=META)
+    del a["q"], a["sink"]
+    _refused(lambda a: dsv4.cache_append(a["pages"], a["rows"], a["table"], a["seq"], a["pos"], a["f"]), a)
+    x, pos, f = _rotary_args()
+    _refused(lambda a: dsv4.rotary_(a["x"], pos, a["f"]), {"x": x, "f": f})
+    _refused(lambda a: dsv4.rotary(x, pos, a["f"]), {"f": f})
+    ids, lens, refs = (torch.empty(n, dtype=torch.int32, device=META) for n in (2, 4, 9))
+    table, pages = _attn_args()["table"], {"pages": _attn_args()["pages"]}
+    _refused(lambda a: dsv4.cache_fork(a["pages"], table, lens, refs, ids, ids), pages)
+    _refused(lambda a: dsv4.cache_compact(a["pages"], table, refs), pages)
+    _refused(lambda a: dsv4.cache_copy(a["pages"], ids, ids), pages)

@@ -39,3 +39,41 @@ def test_rotary_forward_mode(cuda_device, how):
     gx, = torch.autograd.grad(rotary(double, pos, f, **how), double, g, create_graph=True)
     gg, = torch.autograd.grad(gx, g, x)
     assert torch.equal(gg, want)
+
+
+def test_operators_without_a_gradient(cuda_device):
+    """paged_attn, append and rotary_ refuse tensors that require a gradient, take them
+    under no_grad and in inference mode, and give new versions to what they write."""
+    from spark_b200 import kv_cache
+    from spark_b200.rotary import rotary, rotary_
+
+    x, t, pos, f = _rotary_args()
+    pages = torch.randn(4, 16, 128, device="cuda").half()
+    table = torch.tensor([[0, 2], [3, 1]], dtype=torch.int32, device="cuda")
+    rows = torch.randn(2, 128, device="cuda").half()
+    q = torch.randn(2, 8, 128, device="cuda").half()
+    sink = torch.zeros(8, device="cuda")
+    at = torch.tensor([20, 5], device="cuda")
+    need = lambda v: v.clone().requires_grad_()  # noqa: E731
+    for call in (lambda: rotary_(need(x), pos, f), lambda: rotary(x, pos, need(f)),
+                 lambda: kv_cache.append(pages, need(rows), table, None, at),
+                 lambda: kv_cache.append(need(pages), rows, table, None, at),
+                 lambda: kv_cache.paged_attn(need(q), pages, table, None, at, sink, 0.1),
+                 lambda: kv_cache.paged_attn(q, need(pages), table, None, at, sink, 0.1),
+                 lambda: kv_cache.paged_attn(q, pages, table, None, at, need(sink), 0.1)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+        with torch.inference_mode():
+            call()
+    want = kv_cache.paged_attn(q, pages, table, None, at, sink, 0.1)
+    with torch.no_grad():
+        assert torch.equal(kv_cache.paged_attn(need(q), pages, table, None, at, need(sink), 0.1), want)
+    w = need(x)
+    z = (x * w).sum()
+    version = x._version
+    rotary_(x, pos, f)
+    assert x._version == version + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
