@@ -16,6 +16,7 @@
 //                         slot_stride, sf_slot_stride
 //   scalars : float[2]    route_scale, swiglu_limit
 #include <ATen/ATen.h>
+#include <ATen/core/DimVector.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -351,11 +352,26 @@ void check_on(const at::Tensor& t, const at::Tensor& like, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
 }
 
-// An index tensor of the given number of elements as contiguous int32 or int64.
-at::Tensor index_tensor(const at::Tensor& t, const at::Tensor& like, int64_t numel, const char* name) {
+// t's elements stand in the order of `shape`: the same sizes but for axes of one entry, or
+// one axis with all of them.  As many elements in another shape would be taken in the wrong order.
+void check_shape(const at::Tensor& t, at::IntArrayRef shape, const char* name) {
+  at::DimVector have, want;
+  int64_t numel = 1;
+  for (int64_t n : t.sizes())
+    if (n != 1) have.push_back(n);
+  for (int64_t n : shape) {
+    if (n != 1) want.push_back(n);
+    numel *= n;
+  }
+  TORCH_CHECK(t.numel() == numel && (have.size() <= 1 || have == want), name, " must be of shape ", shape, ", is ",
+              t.sizes());
+}
+
+// An index tensor in the order of `shape` as contiguous int32 or int64.
+at::Tensor index_tensor(const at::Tensor& t, const at::Tensor& like, at::IntArrayRef shape, const char* name) {
   check_on(t, like, name);
   TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
-  TORCH_CHECK(t.numel() == numel, name, " must have ", numel, " elements, has ", t.numel());
+  check_shape(t, shape, name);
   return t.contiguous();
 }
 
@@ -363,7 +379,7 @@ at::Tensor index_tensor(const at::Tensor& t, const at::Tensor& like, int64_t num
 // the kernels take as padding or refuse, instead of another sequence's id.
 at::Tensor int32_list(const at::Tensor& t, const at::Tensor& like, const char* name) {
   TORCH_CHECK(t.dim() == 1, name, " must have one dimension");
-  const at::Tensor v = index_tensor(t, like, t.numel(), name);
+  const at::Tensor v = index_tensor(t, like, t.sizes(), name);
   return v.scalar_type() == at::kInt ? v : v.clamp(INT32_MIN, INT32_MAX).to(at::kInt);
 }
 
@@ -393,14 +409,15 @@ at::Tensor four_dims(const at::Tensor& x, bool may_copy) {
   return v;
 }
 
-void run_rotary(const at::Tensor& x, const at::Tensor& y, const at::Tensor& positions, const at::Tensor& freqs,
-                bool interleaved, std::optional<int64_t> offset, bool inverse, double amplitude) {
+// x and y [B, S, H, D]; `tokens`: the sizes in front of heads and channels as the caller has them.
+void run_rotary(const at::Tensor& x, const at::Tensor& y, const at::Tensor& positions, at::IntArrayRef tokens,
+                const at::Tensor& freqs, bool interleaved, std::optional<int64_t> offset, bool inverse, double amplitude) {
   const int dtype = dtype_of(x, "x", true);
   const int rot = rotated_channels(freqs, x);
   const int64_t D = x.size(3), off = offset.value_or(D - rot);
   TORCH_CHECK(off >= 0 && off + rot <= D, "the rotated channels do not fit into a head of ", D);
   for (int i = 0; i < 4; ++i) TORCH_CHECK(x.size(i) <= INT32_MAX, "x is too large");
-  const at::Tensor pos = index_tensor(positions, x, x.size(0) * x.size(1), "positions");
+  const at::Tensor pos = index_tensor(positions, x, tokens, "positions");
   if (x.numel() == 0) return;
   c10::cuda::CUDAGuard guard(x.device());
   long long xs[3], ys[3];
@@ -420,7 +437,7 @@ at::Tensor rotary(const at::Tensor& x, const at::Tensor& positions, const at::Te
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
   const at::Tensor v = four_dims(x, true);
   at::Tensor y = at::empty(v.sizes(), v.options());
-  run_rotary(v, y, positions, freqs, interleaved, offset, inverse, amplitude);
+  run_rotary(v, y, positions, x.sizes().slice(0, x.dim() - 2), freqs, interleaved, offset, inverse, amplitude);
   return y.view(x.sizes());
 }
 
@@ -473,7 +490,7 @@ void rotary_(at::Tensor x, const at::Tensor& positions, const at::Tensor& freqs,
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
   TORCH_CHECK(at::has_internal_overlap(x) != at::MemOverlap::Yes, "x must not overlap itself (expanded tensor)");
   const at::Tensor v = four_dims(x, false);
-  run_rotary(v, v, positions, freqs, interleaved, offset, inverse, amplitude);
+  run_rotary(v, v, positions, x.sizes().slice(0, x.dim() - 2), freqs, interleaved, offset, inverse, amplitude);
 }
 
 // The page tensor as [L, P, page_size, D] with whole pages contiguous.
@@ -674,7 +691,7 @@ at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& pages, const at::Te
   const RowIndex ix = row_index(seq_ids, positions, pages, T, tb.n_seqs);
   at::Tensor sink;
   if (attn_sink.has_value()) {
-    TORCH_CHECK(attn_sink->numel() == H, "attn_sink must have an entry per head");
+    check_shape(*attn_sink, {H}, "attn_sink");
     sink = attn_sink->to(pages.device(), at::kFloat).contiguous();
   }
   at::Tensor out = at::empty({T, H, p.D}, q.options());

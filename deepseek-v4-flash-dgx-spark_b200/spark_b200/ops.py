@@ -19,6 +19,7 @@ A MoE layer crosses the boundary as three lists (``layer_args``):
 
 from __future__ import annotations
 
+import math
 import threading
 
 import torch
@@ -125,18 +126,39 @@ def _register_fakes() -> None:
     def _(x, weight, weight_atoms):
         return x.new_empty((*x.shape[:-1], weight.shape[0]))
 
+    def in_order(t, shape, name):
+        have, want = [n for n in t.shape if n != 1], [n for n in shape if n != 1]
+        if t.numel() != math.prod(shape) or (len(have) > 1 and have != want):
+            raise RuntimeError(f"{name} must be of shape {list(shape)}, is {list(t.shape)}")
+
     @fake("rotary")
     def _(x, positions, freqs, interleaved=True, offset=None, inverse=False, amplitude=1.0):
+        in_order(positions, x.shape[:-2], "positions")
         return x.new_empty(x.shape)
+
+    @fake("rotary_")
+    def _(x, positions, freqs, interleaved=True, offset=None, inverse=False, amplitude=1.0):
+        in_order(positions, x.shape[:-2], "positions")
+
+    @fake("cache_append")
+    def _(pages, rows, page_table, seq_ids, positions, freqs=None, interleaved=True, offset=None, amplitude=1.0):
+        in_order(positions, rows.shape[:1], "positions")
+        if seq_ids is not None:
+            in_order(seq_ids, rows.shape[:1], "seq_ids")
 
     @fake("paged_attn")
     def _(q, pages, page_table, seq_ids, positions, attn_sink, softmax_scale, window=0, first=0):
+        in_order(positions, q.shape[:1], "positions")
+        if seq_ids is not None:
+            in_order(seq_ids, q.shape[:1], "seq_ids")
+        if attn_sink is not None:
+            in_order(attn_sink, q.shape[1:2], "attn_sink")
         return q.new_empty(q.shape)
 
     @fake("cache_compact")
     def _(pages, page_table, page_refs):
         return page_refs.new_empty(page_refs.shape)
 
-    for name in ("rotary_", "cache_append", "cache_reserve", "cache_free", "cache_fork", "cache_copy"):
+    for name in ("cache_reserve", "cache_free", "cache_fork", "cache_copy"):
         torch.library.register_fake(lib + name, lambda *args, **kwargs: None)
 

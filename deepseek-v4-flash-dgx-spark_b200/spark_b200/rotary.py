@@ -54,8 +54,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, int
            offset: int | None = None, inverse: bool = False, amplitude: float = 1.0) -> torch.Tensor:
     """x [..., heads, dim] (bf16, fp16 or fp32, any strides) with the pairs of the
     ``2 * len(freqs)`` channels from ``offset`` on (default: the last ones)
-    turned by ``positions * freqs``, times ``amplitude``; positions [...] int32
-    or int64.  ``inverse`` turns back (the transposed map).  Differentiable in x,
+    turned by ``positions * freqs``, times ``amplitude``; positions [...] (or flat)
+    int32 or int64.  ``inverse`` turns back (the transposed map).  Differentiable in x,
     not in freqs."""
     return ops.load().rotary(x, positions, freqs, interleaved, offset, inverse, float(amplitude))
 

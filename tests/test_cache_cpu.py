@@ -198,3 +198,48 @@ def test_oracle_pool_keeps_counts():
     pool.reserve([4, 5], [16, 12])
     assert pool.short and pool.lens[4] == 0
     assert C.visible(9, 3, 2).tolist() == [0, 1, 7, 8, 9] and C.visible(2, 5, 2).tolist() == [0, 1, 2]
+
+
+def test_index_tensors_of_another_shape_are_refused(dsv4):
+    """As many elements in another order are no positions: those of a transposed batch
+    would turn tokens by other tokens' positions.  Axes of one entry say nothing, and a
+    flat vector has one order only."""
+    m = torch.device("meta")
+
+    def ints(*shape):
+        return torch.empty(*shape, dtype=torch.int64, device=m)
+
+    f = torch.empty(32, dtype=torch.float64, device=m)
+    x = torch.empty(2, 3, 4, 128, device=m)
+    for op in (dsv4.rotary, dsv4.rotary_):
+        for good in ((2, 3), (6,), (2, 1, 3), (1, 6)):
+            op(x, ints(*good), f)
+        for bad in ((3, 2), (1, 3, 2), (2, 3, 2), (5,), (2,)):
+            with pytest.raises(RuntimeError, match="positions"):
+                op(x, ints(*bad), f)
+        op(x[0, 0], ints(1)[0], f)
+        op(x[:0], ints(0, 3), f)
+        five = torch.empty(2, 3, 4, 5, 128, device=m)
+        op(five, ints(2, 3, 4), f)
+        for bad in ((6, 4), (2, 12), (4, 3, 2)):
+            with pytest.raises(RuntimeError, match="positions"):
+                op(five, ints(*bad), f)
+    pages, table = torch.empty(9, 16, 128, dtype=torch.bfloat16, device=m), torch.empty(8, 8, dtype=torch.int32, device=m)
+    q, rows = torch.empty(6, 4, 128, dtype=torch.bfloat16, device=m), torch.empty(6, 128, dtype=torch.bfloat16, device=m)
+
+    def attend(seq=None, pos=ints(6), sink=None):
+        return dsv4.paged_attn(q, pages, table, seq, pos, sink, 0.1)
+
+    def append(seq=None, pos=ints(6)):
+        return dsv4.cache_append(pages, rows, table, seq, pos)
+
+    for call in (attend, append):
+        for good in (dict(), dict(pos=ints(6, 1)), dict(seq=ints(6)), dict(seq=ints(1, 6))):
+            call(**good)
+        for bad in (dict(pos=ints(2, 3)), dict(pos=ints(7)), dict(seq=ints(3, 2)), dict(seq=ints(5))):
+            with pytest.raises(RuntimeError, match="positions|seq_ids"):
+                call(**bad)
+    attend(sink=torch.empty(4, device=m))
+    for bad in ((2, 2), (3,), (4, 4)):
+        with pytest.raises(RuntimeError, match="attn_sink"):
+            attend(sink=torch.empty(*bad, device=m))
