@@ -1076,9 +1076,14 @@ int dsv4_rotary(const void* x, void* y, int dtype, const void* positions, int po
                        x_strides, y_strides, static_cast<cudaStream_t>(stream));
 }
 
+// The kernels step through lists, sequences and pages in 32 bits: a step past the end
+// (1024 entries at most) must not wrap.
+constexpr int kCacheMost = INT_MAX - 4095;  // 2^31 - 4096
+
 // What every entry point on a paged cache asks of its sizes.
 static int cache_shape(int n_pages, int page_size, int n_seqs, int max_pages) {
   if (n_pages <= 0 || page_size <= 0 || n_seqs <= 0 || max_pages <= 0) return DSV4_ERR_ARG;
+  if (n_pages >= kCacheMost || n_seqs >= kCacheMost) return DSV4_ERR_UNSUPPORTED;
   if (page_size > 4096 || max_pages > (1 << 20) || (long long)max_pages * page_size > INT_MAX - 4096)
     return DSV4_ERR_UNSUPPORTED;
   return DSV4_OK;
@@ -1103,6 +1108,7 @@ int dsv4_cache_append(const void* rows, long long row_stride, int dtype, int T, 
   if (rc == DSV4_OK) rc = cache_rows(pages, 1, page_size, D, 0, page_stride);
   if (rc != DSV4_OK) return rc;
   if (rot > 2 * kAppendPairs) return DSV4_ERR_UNSUPPORTED;
+  if (T >= kCacheMost) return DSV4_ERR_UNSUPPORTED;
   if (T == 0) return DSV4_OK;
   if (!rows || !page_table || !positions || (rot && !freqs)) return DSV4_ERR_ARG;
   bind_device(pages);
@@ -1121,6 +1127,7 @@ int dsv4_cache_reserve(int* page_table, int* seq_lens, int* page_refs, int n_seq
   if (n < 0) return DSV4_ERR_ARG;
   const int rc = cache_shape(n_pages, page_size, n_seqs, max_pages);
   if (rc != DSV4_OK) return rc;
+  if (n >= kCacheMost) return DSV4_ERR_UNSUPPORTED;
   if (n == 0) return DSV4_OK;
   if (!page_table || !seq_lens || !page_refs || !seqs || !new_lens) return DSV4_ERR_ARG;
   if (!workspace || workspace_bytes < cache_reserve_workspace(n, n_seqs, n_pages)) return DSV4_ERR_WORKSPACE;
@@ -1134,6 +1141,7 @@ int dsv4_cache_free(int* page_table, int* seq_lens, int* page_refs, int n_seqs, 
   if (n < 0) return DSV4_ERR_ARG;
   const int rc = cache_shape(n_pages, 1, n_seqs, max_pages);
   if (rc != DSV4_OK) return rc;
+  if (n >= kCacheMost) return DSV4_ERR_UNSUPPORTED;
   if (n == 0) return DSV4_OK;
   if (!page_table || !seq_lens || !page_refs || !seqs) return DSV4_ERR_ARG;
   bind_device(page_table);
@@ -1153,6 +1161,7 @@ int dsv4_cache_fork(void* pages, int n_layers, int D, long long layer_stride, lo
   int rc = cache_shape(n_pages, page_size, n_seqs, max_pages);
   if (rc == DSV4_OK) rc = cache_rows(pages, n_layers, page_size, D, layer_stride, page_stride);
   if (rc != DSV4_OK) return rc;
+  if (n >= kCacheMost) return DSV4_ERR_UNSUPPORTED;
   if (n == 0) return DSV4_OK;
   if (!page_table || !seq_lens || !page_refs || !parents || !children) return DSV4_ERR_ARG;
   if (!workspace || workspace_bytes < cache_fork_workspace(n, n_seqs)) return DSV4_ERR_WORKSPACE;
@@ -1186,6 +1195,7 @@ int dsv4_cache_copy(void* pages, int n_layers, int D, long long layer_stride, lo
   int rc = cache_shape(n_pages, page_size, 1, 1);
   if (rc == DSV4_OK) rc = cache_rows(pages, n_layers, page_size, D, layer_stride, page_stride);
   if (rc != DSV4_OK) return rc;
+  if (n >= kCacheMost) return DSV4_ERR_UNSUPPORTED;
   if (n == 0) return DSV4_OK;
   if (!src || !dst) return DSV4_ERR_ARG;
   bind_device(pages);

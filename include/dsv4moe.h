@@ -318,7 +318,8 @@ DSV4_API int dsv4_rotary(const void* x, void* y, int dtype, const void* position
  * the last), seq_lens int32 [n_seqs] (tokens a sequence has room for), page_refs
  * int32 [n_pages] (sequences that hold a page; 0 = free).  Tables live on the
  * device and change in stream order; nothing is read back.  Bad entries are
- * skipped and latch DSV4_DEVERR_BAD_CACHE_INDEX.
+ * skipped and latch DSV4_DEVERR_BAD_CACHE_INDEX.  n_seqs, n_pages and the number
+ * of entries or rows of a call stay below 2^31 - 4096 (DSV4_ERR_UNSUPPORTED).
  *
  * append: row t of rows [T,D] (row_stride elements apart) is rotated (rot = 0:
  * not) and written as row positions[t] of sequence seq_ids[t] (NULL: sequence
@@ -345,9 +346,9 @@ DSV4_API int dsv4_cache_free(int* page_table, int* seq_lens, int* page_refs, int
 /* fork: the empty sequence children[i] becomes the first fork_lens[i] tokens
  * (NULL: all) of parents[i].  Full pages are shared; a part-filled last page is
  * copied to a free page (lowest id first) in every layer, so either side may go
- * on writing behind the fork (not before it: those pages are the other's too).  A child that holds tokens or is named again, or a
- * length beyond the parent's, is a bad entry; a negative id is padding; too few
- * free pages change nothing. */
+ * on writing behind the fork (not before it: those pages are the other's too).  A
+ * child that holds tokens or is named again, or a length beyond the parent's, is
+ * a bad entry; a negative id is padding; too few free pages change nothing. */
 DSV4_API long long dsv4_cache_fork_workspace_bytes(int n, int n_seqs);
 DSV4_API int dsv4_cache_fork(void* pages, int n_layers, int D, long long layer_stride, long long page_stride,
                              int* page_table, int* seq_lens, int* page_refs, int n_seqs, int max_pages, int n_pages,

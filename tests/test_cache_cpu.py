@@ -243,3 +243,37 @@ def test_index_tensors_of_another_shape_are_refused(dsv4):
     for bad in ((2, 2), (3,), (4, 4)):
         with pytest.raises(RuntimeError, match="attn_sink"):
             attend(sink=torch.empty(*bad, device=m))
+
+
+def test_sizes_at_the_end_of_32_bits_are_refused(lib):
+    """The page operations step through lists, sequences and pages by up to a block's
+    threads in 32 bits: a step past the end must not wrap, or the loop never ends."""
+    from spark_b200 import _lib
+
+    big, most, huge = 1 << 62, 2 ** 31 - 1, 2 ** 31 - 4096
+
+    def reserve(n_seqs=4, n_pages=16, n=2):
+        return lib.dsv4_cache_reserve(P, P, P, n_seqs, 8, n_pages, 64, P, P, n, P, big, None)
+
+    def free(n_seqs=4, n_pages=16, n=2):
+        return lib.dsv4_cache_free(P, P, P, n_seqs, 8, n_pages, P, n, None)
+
+    def fork(n_seqs=4, n_pages=16, n=2):
+        return lib.dsv4_cache_fork(P, 1, 512, 1 << 24, 64 * 512, P, P, P, n_seqs, 8, n_pages, 64, P, P, None, n, P, big, None)
+
+    def compact(n_seqs=4, n_pages=16):
+        return lib.dsv4_cache_compact(P, 1, 512, 1 << 24, 64 * 512, P, P, n_seqs, 8, n_pages, 64, P, P, big, None)
+
+    def copy(n_pages=16, n=2):
+        return lib.dsv4_cache_copy(P, 1, 512, 1 << 24, 64 * 512, n_pages, 64, P, P, n, None)
+
+    def append(n_seqs=4, n_pages=16, T=2):
+        return lib.dsv4_cache_append(P, 512, 0, T, 512, P, n_pages, 64, 64 * 512, P, n_seqs, 8, None, P, 0, None, 0, 0, 1,
+                                     1.0, None)
+
+    for call, names in ((reserve, ("n_seqs", "n_pages", "n")), (free, ("n_seqs", "n_pages", "n")),
+                        (fork, ("n_seqs", "n_pages", "n")), (compact, ("n_seqs", "n_pages")), (copy, ("n_pages", "n")),
+                        (append, ("n_seqs", "n_pages", "T"))):
+        for name in names:
+            for size in (most, huge):
+                assert call(**{name: size}) == _lib.ERR_UNSUPPORTED, (call.__name__, name, size)
