@@ -520,7 +520,11 @@ Pages pages_of(const at::Tensor& pages, bool one_layer) {
   // the stride of a dimension of one entry says nothing
   p.page_stride = p.n_pages > 1 ? pages.stride(d - 3) : static_cast<long long>(p.page_size) * p.D;
   p.layer_stride = p.layers > 1 ? pages.stride(0) : 0;
-  TORCH_CHECK(p.layers == 1 || p.layer_stride != 0, "layers must not overlap");
+  // layers outermost, or the layers of a page side by side
+  const long long page = static_cast<long long>(p.page_size) * p.D;
+  TORCH_CHECK(p.layers == 1 || p.layer_stride >= (p.n_pages - 1) * p.page_stride + page ||
+                  (p.layer_stride >= page && (p.n_pages == 1 || p.page_stride >= (p.layers - 1) * p.layer_stride + page)),
+              "layers must not overlap");
   return p;
 }
 

@@ -37,3 +37,30 @@ def test_positions_and_ids_of_another_shape(cuda_device):
                  lambda: kv_cache.paged_attn(q, pages, table, seq, at, sink.view(2, 2), 0.1)):
         with pytest.raises(RuntimeError, match="must be of shape"):
             call()
+
+
+def test_layers_that_overlap(cuda_device):
+    """Layers apart by less than their pages, or pages by less than their layers, would be
+    copied onto one another; nested layouts of either order are taken."""
+    from spark_b200 import _lib, kv_cache
+
+    base = torch.randn(4096, device="cuda").half()
+    src, dst = (torch.tensor([v], dtype=torch.int32, device="cuda") for v in (0, 2))
+    page = 4 * 8
+    for strides in ((96, 32), (160, 40), (32, 96), (48, 160), (1000, 32)):      # three layers, three pages
+        v = base.clone().as_strided((3, 3, 4, 8), (*strides, 8, 1))
+        want = v.clone()
+        want[:, 2] = want[:, 0]
+        kv_cache.copy_pages(v, src, dst)
+        torch.cuda.synchronize()
+        _lib.raise_on_device_error()
+        assert torch.equal(v, want)
+    for strides in ((0, 32), (88, 32), (32, 64), (24, 96), (40, 104), (16, 32), (32, 0), (104, 40), (64, 32)):
+        v = base.as_strided((3, 3, 4, 8), (*strides, 8, 1))
+        for call in (lambda: kv_cache.copy_pages(v, src, dst),
+                     lambda: kv_cache.compact(v, torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                                              torch.ones(3, dtype=torch.int32, device="cuda"))):
+            with pytest.raises(RuntimeError, match="must not overlap"):
+                call()
+    one = base.clone().as_strided((3, 1, 4, 8), (page, 7, 8, 1))                # one page a layer
+    kv_cache.copy_pages(one, src, src)
