@@ -246,3 +246,23 @@ def test_argument_checks(cuda_device):
     kv_cache.free(*ok, _ints([]))
     kv_cache.reserve(*ok, _ints([]), _ints([]), 16)
     c.same()
+
+
+@pytest.mark.parametrize("n,layers", [(3001, 11), (17000, 3)])  # a part of the layers per block, all of them
+def test_many_copies(cuda_device, n, layers):
+    from spark_b200 import _lib, kv_cache
+
+    g = torch.Generator(device="cuda").manual_seed(n)
+    pages = torch.randn(layers, 2 * n + 5, 2, 16, generator=g, device="cuda").bfloat16()
+    order = torch.randperm(2 * n + 5, generator=g, device="cuda").int()
+    src, dst = order[:n].clone(), order[n:2 * n].clone()
+    src[7], dst[11] = -1, src[40]                                     # padding; another entry's source
+    live = torch.ones(n, dtype=torch.bool, device="cuda")
+    live[7] = live[11] = False
+    want = pages.clone()
+    want[:, dst[live].long()] = want[:, src[live].long()]
+    kv_cache.copy_pages(pages, src, dst)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cache sequence, position"):
+        _lib.raise_on_device_error()
+    assert torch.equal(pages, want)
