@@ -893,7 +893,8 @@ int64_t read_into(int64_t fd, at::Tensor& destination, int64_t size, int64_t off
 // so that a backward pass which saved one of them is refused.
 template <typename Tuple, size_t... i>
 void bump_versions(const Tuple& args, std::index_sequence<i...>) {
-  (torch::autograd::impl::bump_version(std::get<i>(args)), ...);
+  // a tensor made in inference mode has no version, and may be written outside of it too
+  ((std::get<i>(args).is_inference() ? void() : torch::autograd::impl::bump_version(std::get<i>(args))), ...);
 }
 
 template <const char* kName, size_t kWritten, typename F>

@@ -1,6 +1,8 @@
 """How the attention cache's operators answer torch's autograd, on meta tensors: what
 is shared by every device lies above the kernels."""
 
+import contextlib
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
@@ -34,18 +36,21 @@ def test_rotary_has_a_tangent(dsv4):
     assert y.shape == t.shape == x.shape
 
 
-def _calls(op):
-    """Every operator that writes: the call, and the tensors it writes."""
+def _calls(op, made=contextlib.nullcontext):
+    """Every operator that writes: the call, and the tensors it writes, which come into
+    being under ``made``."""
     def ints(*shape):
         return torch.empty(*shape, dtype=torch.int32, device=META)
 
     def bf16(*shape):
         return torch.empty(*shape, dtype=torch.bfloat16, device=META)
 
-    x, pos, f = _rotary_args()
-    pages, table, lens, refs, ids = bf16(2, 9, 16, 64), ints(4, 8), ints(4), ints(9), ints(2)
-    rows, f16 = bf16(2, 64), torch.empty(16, dtype=torch.float64, device=META)
-    layer = pages[0]
+    with made():
+        x = _rotary_args()[0]
+        pages, table, lens, refs = bf16(2, 9, 16, 64), ints(4, 8), ints(4), ints(9)
+        layer = pages[0]
+    _, pos, f = _rotary_args()
+    rows, ids, f16 = bf16(2, 64), ints(2), torch.empty(16, dtype=torch.float64, device=META)
     return {
         "rotary_": (lambda: op.rotary_(x, pos, f), [x]),
         "cache_append": (lambda: op.cache_append(layer, rows, table, ids, ids, f16), [pages]),
@@ -127,3 +132,14 @@ def test_operators_without_a_gradient_refuse_one(dsv4):
     _refused(lambda a: dsv4.cache_fork(a["pages"], table, lens, refs, ids, ids), pages)
     _refused(lambda a: dsv4.cache_compact(a["pages"], table, refs), pages)
     _refused(lambda a: dsv4.cache_copy(a["pages"], ids, ids), pages)
+
+
+@pytest.mark.parametrize("name", WRITING)
+def test_tensors_made_in_inference_mode_are_written_outside_of_it(dsv4, name):
+    """A cache made in inference mode has no versions to raise; beside ordinary ids and
+    positions it is written outside of inference mode too."""
+    call, written = _calls(dsv4, torch.inference_mode)[name]
+    assert all(t.is_inference() for t in written)
+    with torch.no_grad():
+        call()
+    call()

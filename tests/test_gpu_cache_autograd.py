@@ -77,3 +77,25 @@ def test_operators_without_a_gradient(cuda_device):
     assert x._version == version + 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         z.backward()
+
+
+def test_a_cache_made_in_inference_mode(cuda_device):
+    """It is written and read outside of inference mode as well."""
+    from spark_b200 import _lib
+    from spark_b200.kv_cache import PagedKVCache
+
+    with torch.inference_mode():
+        cache = PagedKVCache(2, 8, 3, 64, page_size=16, dim=128)
+    ids, pos = torch.arange(2, device="cuda").int(), torch.tensor([3, 17], device="cuda").int()
+    rows = torch.randn(2, 128, device="cuda").bfloat16()
+    cache.reserve(ids, pos + 1)
+    cache.append(1, rows, ids, pos)
+    cache.fork(ids[1:], ids[1:] + 1)
+    q = torch.randn(1, 4, 128, device="cuda").bfloat16()
+    out = cache.attend(1, q, ids[1:] + 1, pos[1:], None, 0.1, window=1)
+    assert torch.equal(out[0], rows[1:].expand(4, 128))               # the only visible row, copied by the fork
+    cache.copy_pages(ids[:1], ids[:1] + 7)
+    cache.free(ids[:1])
+    assert cache.compact().tolist()[1:4] == [1, 2, 0]
+    torch.cuda.synchronize()
+    _lib.raise_on_device_error()
