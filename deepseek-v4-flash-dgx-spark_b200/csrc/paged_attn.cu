@@ -23,10 +23,12 @@
 // (measured), 1970 cycles per chunk, against 2840 at which an SM's share of HBM
 // delivers the chunk's 64 KB.  What is left is the ring: shared memory holds Q (64 KB)
 // and 2.25 chunks, and a stage comes back only after its load (about 2000 cycles), its
-// chunk's softmax (1250) and both products, a period of 2850 to 3000 cycles.  Measured:
-// 5.5 TB/s (0.85 of the copy rate) between 40000 and 80000 keys of 16 rows, 5.0 TB/s
-// over whole calls (16 rows of 60000 keys: 193 us), of which about 17 us are start,
-// output and join.  Chunks of 128 keys cost fewer tensor cycles per key but hold all of
+// chunk's softmax (1250) and both products, a period of 2850 to 3000 cycles.  Shared
+// memory is not far from its own rate either: a chunk moves about 296 KB through it (Q 64,
+// the keys 64 for each product, the weights 4 x 8, the load 64, the weights' stores 8),
+// 2310 cycles at 128 bytes each.  Measured over whole calls, 16 rows of 40000, 60000 and
+// 80000 keys: 138, 194 and 254 us, 4.75, 5.05 and 5.15 TB/s (0.73 to 0.80 of the copy rate),
+// of which about 20 us are start, output and join.  Chunks of 128 keys cost fewer tensor cycles per key but hold all of
 // the ring until their softmax is done, and the loads stand still for half of the time
 // (16 rows of up to 131072 keys: 353 against 291 us at that step).
 //
