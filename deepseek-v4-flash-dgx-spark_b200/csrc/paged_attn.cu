@@ -18,19 +18,20 @@
 // heads' running max and sum in registers and takes their scores from one
 // tcgen05.ld.16x256b (M = 64 fills 16 lanes of each TMEM quarter).
 //
-// Bound: a row of D = 512 is 1 KB from HBM and 131 kFLOP with 64 heads.  Issued
-// from warp-uniform code the two products cost 36 and 51 cycles per instruction
-// (measured), 1970 cycles per chunk, against 2840 at which an SM's share of HBM
-// delivers the chunk's 64 KB.  What is left is the ring: shared memory holds Q (64 KB)
-// and 2.25 chunks, and a stage comes back only after its load (about 2000 cycles), its
-// chunk's softmax (1250) and both products, a period of 2850 to 3000 cycles.  Shared
-// memory is not far from its own rate either: a chunk moves about 296 KB through it (Q 64,
-// the keys 64 for each product, the weights 4 x 8, the load 64, the weights' stores 8),
-// 2310 cycles at 128 bytes each.  Measured over whole calls, 16 rows of 40000, 60000 and
-// 80000 keys: 138, 194 and 254 us, 4.75, 5.05 and 5.15 TB/s (0.73 to 0.80 of the copy rate),
-// of which about 20 us are start, output and join.  Chunks of 128 keys cost fewer tensor cycles per key but hold all of
-// the ring until their softmax is done, and the loads stand still for half of the time
-// (16 rows of up to 131072 keys: 353 against 291 us at that step).
+// Bound: a row of D = 512 is 1 KB from HBM and 131 kFLOP with 64 heads.  Issued from
+// warp-uniform code the two products cost 36 and 51 cycles per instruction (measured),
+// 1970 cycles per chunk, against 2840 at which an SM's share of HBM delivers the chunk's
+// 64 KB.  What is left is the ring: shared memory holds Q (64 KB) and 2.25 chunks, and a
+// stage comes back only after its load (about 2000 cycles), its chunk's softmax (1250)
+// and both products, a period of 2850 to 3000 cycles.  Shared memory is not far from its
+// own rate either: a chunk moves about 296 KB through it (Q 64, the keys 64 for each
+// product, the weights 4 x 8, the load 64, the weights' stores 8), 2310 cycles at 128
+// bytes each.  Measured over whole calls, 16 rows of 40000, 60000 and 80000 keys: 138,
+// 194 and 254 us, 4.75, 5.05 and 5.15 TB/s (0.73 to 0.80 of the copy rate), of which
+// about 20 us are start, output and join.  Chunks of 128 keys cost fewer tensor cycles
+// per key but hold all of the ring until their softmax is done, and the loads stand
+// still for half of the time (16 rows of up to 131072 keys: 353 against 291 us at that
+// step).
 //
 // Work split: the visible keys of all rows, in boxes of up to 64 keys on one page,
 // form one list, and the list is cut into equal shares, one per CTA (one CTA per
@@ -69,14 +70,15 @@ constexpr int kPaSnapChunks = 3;                  // a border moves so far to a 
 constexpr float kPaNoMax = -3.402823466e38f;      // running max of a piece before its first finite score
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Weights are 2^(score - m), scores in base 2.  m is set to `lift` below the largest score so
-// far, and again only once a score passes m by lift + headroom, so the largest weight of
-// a row lies between 2^lift and 2^(lift + headroom).  bf16 has fp32's range and needs no
-// lift.  fp16 ends at 2^16 and counts in steps of 2^-24 below 2^-14: with the lift a key
-// keeps all bits of its weight down to 2^-23 of the largest one and some down to 2^-34,
-// which counts where one dominating key of small values stands before many others.  A
-// lift of 12 and 3 of headroom would keep three more bits, but the output is rescaled more often (64
-// ragged rows of 64 fp16 heads 84.0 us at lift 5, 84.8 at 9, 87.8 at 12).
+// Weights are 2^(score - m), scores in base 2.  m is set to `lift` below the largest
+// score so far, and again only once a score passes m by lift + headroom, so the largest
+// weight of a row lies between 2^lift and 2^(lift + headroom).  bf16 has fp32's range
+// and needs no lift.  fp16 ends at 2^16 and counts in steps of 2^-24 below 2^-14: with
+// the lift a key keeps all bits of its weight down to 2^-23 of the largest one and some
+// down to 2^-34, which counts where one dominating key of small values stands before
+// many others.  A lift of 12 and 3 of headroom would keep three more bits, but the
+// output is rescaled more often (64 ragged rows of 64 fp16 heads 84.0 us at lift 5, 84.8
+// at 9, 87.8 at 12).
 template <typename T>
 struct PaWeight {
   static constexpr float lift = 0.f, headroom = 10.f;
